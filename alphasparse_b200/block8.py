@@ -1,0 +1,142 @@
+"""Block-sparse matrices in 8 bits, rows in 8 bits, their products and gradients (include/asp_b200_block8.h).
+
+Everything takes device pointers (ints) and runs on the stream of its Context, like PlanGroup.spmv; types are "f32", "f16" and
+"bf16". `ld` is the distance of two rows in elements, 0 for rows that lie side by side.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import capi, graph
+
+BLOCK = 128
+APPLY_ROWS = 32  # most rows of Block8.apply
+TYPES = {"f32": capi.F32, "f16": 6, "bf16": 7}
+
+EXPORTS = [
+    "asp_rows8_create", "asp_rows8_destroy", "asp_rows8_quantize", "asp_rows8_restore", "asp_rows8_count", "asp_block8_create", "asp_block8_from_matrix",
+    "asp_block8_destroy", "asp_block8_blocks", "asp_block8_pattern", "asp_block8_bytes", "asp_block8_set_values", "asp_block8_get_values", "asp_block8_apply",
+    "asp_block8_product", "asp_block8_gradient",
+]
+
+_bound = None
+
+
+def _lib():
+    global _bound
+    if _bound is None:
+        L = capi.lib()
+        p, u64, i32, out = C.c_void_p, C.c_uint64, C.c_int, C.POINTER(C.c_void_p)
+        for name, args, result in (
+            ("asp_rows8_create", [p, u64, u64, out], i32), ("asp_rows8_destroy", [p], None), ("asp_rows8_quantize", [p, p, p, i32, u64, u64], i32),
+            ("asp_rows8_restore", [p, p, p, i32, u64], i32), ("asp_rows8_count", [p], u64), ("asp_block8_create", [p, u64, u64, p, p, i32, out], i32),
+            ("asp_block8_from_matrix", [p, p, i32, out], i32), ("asp_block8_destroy", [p], None), ("asp_block8_blocks", [p], u64),
+            ("asp_block8_pattern", [p, p, p], i32), ("asp_block8_bytes", [p], u64), ("asp_block8_set_values", [p, p, p, i32], i32),
+            ("asp_block8_get_values", [p, p, p], i32), ("asp_block8_apply", [p, p, i32, p, i32, u64, u64, p, i32, u64], i32),
+            ("asp_block8_product", [p, p, i32, p, p, i32, u64], i32), ("asp_block8_gradient", [p, p, p, p, i32, u64, p, i32], i32),
+        ):
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = args, result
+        _bound = L
+    return _bound
+
+
+class Rows8:
+    """asp_rows8: up to max_rows rows of n_cols columns in 8 bits, a scale for each row and 128 columns."""
+
+    def __init__(self, ctx: capi.Context, max_rows: int, n_cols: int):
+        self._h = C.c_void_p()
+        self.ctx, self.max_rows, self.n_cols = ctx, max_rows, n_cols
+        capi.check(_lib().asp_rows8_create(ctx.handle, max_rows, n_cols, C.byref(self._h)))
+
+    def __len__(self) -> int:
+        """Rows held."""
+        return int(_lib().asp_rows8_count(self._h))
+
+    def quantize(self, x: int, n: int, dtype: str, ld: int = 0) -> None:
+        """n rows at x to 8 bits."""
+        capi.check(_lib().asp_rows8_quantize(self.ctx.handle, self._h, x, TYPES[dtype], n, ld))
+
+    def restore(self, out: int, dtype: str, ld: int = 0) -> None:
+        """What the rows held stand for."""
+        capi.check(_lib().asp_rows8_restore(self.ctx.handle, self._h, out, TYPES[dtype], ld))
+
+    def close(self):
+        if self._h:
+            _lib().asp_rows8_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Block8:
+    """asp_block8: an n_rows x n_cols matrix of which 128 x 128 blocks are stored, in 8 bits with a scale each. block_ptr, block_col:
+    the blocks by block row, as in CSR. transposed: products with the transposed matrix are wanted, too."""
+
+    def __init__(self, ctx: capi.Context, n_rows: int, n_cols: int, block_ptr, block_col, transposed: bool = False):
+        ptr = np.ascontiguousarray(block_ptr, dtype=np.int64)
+        col = np.ascontiguousarray(block_col, dtype=np.uint32)
+        if ptr.ndim != 1 or ptr.shape[0] != -(-n_rows // BLOCK) + 1 or col.ndim != 1 or (ptr[-1] != col.shape[0]):
+            raise ValueError("block_ptr has an entry for each block row and one more, the last of them the number of blocks")
+        h = C.c_void_p()
+        capi.check(_lib().asp_block8_create(ctx.handle, n_rows, n_cols, ptr.ctypes.data, col.ctypes.data, int(transposed), C.byref(h)))
+        self._take(ctx, h, n_rows, n_cols)
+
+    @classmethod
+    def from_matrix(cls, ctx: capi.Context, matrix: graph.Matrix, transposed: bool = False) -> "Block8":
+        """The blocks of `matrix` that have an entry, with its values."""
+        self = cls.__new__(cls)
+        h = C.c_void_p()
+        capi.check(_lib().asp_block8_from_matrix(ctx.handle, matrix._h, int(transposed), C.byref(h)))
+        self._take(ctx, h, *matrix.shape)
+        return self
+
+    def _take(self, ctx, h, n_rows, n_cols):
+        self._h, self.ctx, self.n_rows, self.n_cols = h, ctx, n_rows, n_cols
+        self.n_blocks = int(_lib().asp_block8_blocks(h))
+
+    def pattern(self):
+        """(block_ptr, block_col)"""
+        ptr, col = np.zeros(-(-self.n_rows // BLOCK) + 1, dtype=np.int64), np.zeros(self.n_blocks, dtype=np.uint32)
+        capi.check(_lib().asp_block8_pattern(self._h, ptr.ctypes.data, col.ctypes.data))
+        return ptr, col
+
+    def bytes(self) -> int:
+        return int(_lib().asp_block8_bytes(self._h))
+
+    def set_values(self, values: int, dtype: str) -> None:
+        """New values of all stored blocks, [n_blocks, 128, 128]."""
+        capi.check(_lib().asp_block8_set_values(self.ctx.handle, self._h, values, TYPES[dtype]))
+
+    def get_values(self, values: int) -> None:
+        """What the stored blocks stand for, [n_blocks, 128, 128] in 32 bits."""
+        capi.check(_lib().asp_block8_get_values(self.ctx.handle, self._h, values))
+
+    def apply(self, x: int, n: int, x_dtype: str, y: int, y_dtype: str, ldx: int = 0, ldy: int = 0, transposed: bool = False) -> None:
+        """y = A x (transposed: A^T x) for n <= 32 rows x in 16 or 32 bits, converted to 8 bits on the way."""
+        capi.check(_lib().asp_block8_apply(self.ctx.handle, self._h, transposed, x, TYPES[x_dtype], n, ldx, y, TYPES[y_dtype], ldy))
+
+    def product(self, x: Rows8, y: int, dtype: str, ld: int = 0, transposed: bool = False) -> None:
+        """y = A x (transposed: A^T x) for the rows that x holds."""
+        capi.check(_lib().asp_block8_product(self.ctx.handle, self._h, transposed, x._h, y, TYPES[dtype], ld))
+
+    def gradient(self, x: Rows8, dy: int, dtype: str, out: int, ld: int = 0, accumulate: bool = False) -> None:
+        """The gradient by the stored blocks, [n_blocks, 128, 128] in 32 bits, from dy and the rows x kept in 8 bits."""
+        capi.check(_lib().asp_block8_gradient(self.ctx.handle, self._h, x._h, dy, TYPES[dtype], ld, out, int(accumulate)))
+
+    def close(self):
+        if self._h:
+            _lib().asp_block8_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

@@ -1,0 +1,128 @@
+// Device side of the 8-bit types of asp_b200_block8.h: scales, rounding, loads and stores of the caller's types.
+#ifndef ASP_BLOCK8_DEVICE_H
+#define ASP_BLOCK8_DEVICE_H
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace asp
+{
+namespace block8
+{
+// |v| where it is finite, else 0
+__device__ __forceinline__ float finite_size(float v)
+{
+    v = fabsf(v);
+    return v < __int_as_float(0x7f800000) ? v : 0.f;
+}
+
+// Exponent + 127 of the scale: the smallest k >= -126 with most <= 448 * 2^k. 448 = 1.75 * 2^8, so k is most's own exponent less 8, and one
+// more where its fraction is above 0.75. (Subnormal `most`: exponent field 0, far below the smallest k.)
+__device__ __forceinline__ unsigned scale_of(float most)
+{
+    const unsigned bits = __float_as_uint(most);
+    const int k = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return (unsigned)max(k, 1);
+}
+__device__ __forceinline__ float power(unsigned scale) { return __uint_as_float(scale << 23); }            // 2^k
+__device__ __forceinline__ float inverse(unsigned scale) { return __uint_as_float((254u - scale) << 23); } // 2^-k; scale is 1 to 247
+
+// Two elements to e4m3, `a` in the low byte. The conversion saturates: what is infinite is made NaN first (v - v is NaN then, else 0).
+__device__ __forceinline__ unsigned pack2(float a, float b, float inv)
+{
+    unsigned short r;
+    a = __fmaf_rn(a, inv, a - a);
+    b = __fmaf_rn(b, inv, b - b);
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ unsigned pack4(const float *v, float inv) { return pack2(v[0], v[1], inv) | pack2(v[2], v[3], inv) << 16; }
+
+// two e4m3 (exact in fp16, NaN included)
+__device__ __forceinline__ __half2 unpack2(unsigned two)
+{
+    unsigned h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)two));
+    return *reinterpret_cast<__half2 *>(&h);
+}
+__device__ __forceinline__ void unpack4(unsigned four, float *v)
+{
+    const float2 a = __half22float2(unpack2(four & 0xffffu)), b = __half22float2(unpack2(four >> 16));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 16 elements that begin on a 16-byte boundary
+template <class T> __device__ __forceinline__ void load16(const T *p, float *v)
+{
+    constexpr int per = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / per; i++)
+    {
+        const uint4 w = *reinterpret_cast<const uint4 *>(p + i * per);
+        const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+        for (int j = 0; j < per; j++) v[i * per + j] = to_float(e[j]);
+    }
+}
+template <class T> __device__ __forceinline__ void store16(T *p, const float *v)
+{
+    constexpr int per = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / per; i++)
+    {
+        uint4 w;
+        T *e = reinterpret_cast<T *>(&w);
+#pragma unroll
+        for (int j = 0; j < per; j++) e[j] = from_float<T>(v[i * per + j]);
+        *reinterpret_cast<uint4 *>(p + i * per) = w;
+    }
+}
+
+// The 16 elements that lane `lane8` of 8 has of a row's block of 128 columns. vec: the row begins on a 16-byte boundary and has the whole block; they are
+// columns 16 * lane8 + i, otherwise 8 * i + lane8, so that the eight lanes read side by side, with zeros behind the row's end.
+template <class T> __device__ __forceinline__ void load_block(const T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec, float *v)
+{
+    if (vec) load16(row + col0 + 16 * lane8, v);
+    else
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+        {
+            const unsigned c = col0 + 8 * i + lane8;
+            v[i] = c < n_cols ? to_float(row[c]) : 0.f;
+        }
+}
+// the largest finite magnitude of what the eight lanes of a block have; all lanes of the warp take part
+__device__ __forceinline__ float largest_of_8(const float *v)
+{
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) most = fmaxf(most, finite_size(v[i]));
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    return most;
+}
+// what load_block gave, to 8 bits; `to` is the block's first byte, vec as in load_block (and the block inside the row)
+__device__ __forceinline__ void store_block(const float *v, bool vec, unsigned lane8, unsigned scale, uint8_t *to)
+{
+    const float inv = inverse(scale);
+    if (vec) *reinterpret_cast<uint4 *>(to + 16 * lane8) = make_uint4(pack4(v, inv), pack4(v + 4, inv), pack4(v + 8, inv), pack4(v + 12, inv));
+    else
+#pragma unroll
+        for (int i = 0; i < 16; i += 2)
+        {
+            const unsigned two = pack2(v[i], v[i + 1], inv);
+            to[8 * i + lane8] = (uint8_t)two;
+            to[8 * (i + 1) + lane8] = (uint8_t)(two >> 8);
+        }
+}
+} // namespace block8
+} // namespace asp
+#endif

@@ -1,0 +1,396 @@
+// Block-sparse 8-bit matrices (asp_b200_block8.h): conversions to and from 8 bits, products with a few rows.
+#include "../../include/asp_b200.h"
+#include "block8.h"
+#include "block8_device.h"
+#include "launch.h"
+
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+namespace asp
+{
+namespace
+{
+using namespace block8;
+
+template <class F> cudaError_t by_type(int dtype, F f)
+{
+    if (dtype == ASP_F32) return f(float());
+    if (dtype == ASP_F16) return f(__half());
+    return f(__nv_bfloat16());
+}
+template <class T> bool vectors(const Dense &x) { return ((uintptr_t)x.p & 15) == 0 && (x.ld * sizeof(T)) % 16 == 0; }
+
+// ---- rows ----------------------------------------------------------------------------------------------------------
+
+// 32 rows x 512 columns to a CTA of 8 warps: a warp takes a row's four blocks at once, 8 lanes and 16 elements a lane each, so that an
+// element is read once and its block's largest is known after three exchanges. Bounded by memory. The scales of a block column
+// are collected so that they leave as 32 bytes in a row instead of one by one.
+constexpr int kQuantRows = 32;
+template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const T *x, uint64_t ld, bool vec, unsigned n, Rows8Dev out)
+{
+    __shared__ uint8_t scales[4][kQuantRows];
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (out.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
+    const unsigned blk0 = blockIdx.x % fours * 4, blk = blk0 + lane / 8, row0 = blockIdx.x / fours * kQuantRows;
+#pragma unroll
+    for (int i = 0; i < kQuantRows / 8; i++)
+    {
+        const unsigned row = row0 + i * 8 + warp;
+        if (row >= n) break;
+        const bool there = blk < n_blocks, together = vec && (blk + 1) * 128 <= out.n_cols;
+        float v[16];
+        load_block(x + (uint64_t)row * ld, blk * 128, out.n_cols, lane8, together, v); // (zeros behind the last block)
+        const float most = largest_of_8(v);
+        if (!there) continue;
+        const unsigned scale = scale_of(most);
+        store_block(v, together, lane8, scale, out.values + (uint64_t)row * out.ld + blk * 128);
+        if (lane8 == 0) scales[lane / 8][i * 8 + warp] = (uint8_t)scale;
+    }
+    __syncthreads();
+    const unsigned b = threadIdx.x / kQuantRows, r = threadIdx.x % kQuantRows;
+    if (b < 4 && blk0 + b < n_blocks && row0 + r < n) out.scales[(uint64_t)(blk0 + b) * out.ld_scales + row0 + r] = scales[b][r];
+}
+
+// 16 columns to a thread, a block of 128 columns and 32 rows to a CTA
+template <class T> __global__ void __launch_bounds__(256) k_rows8_restore(Rows8Dev x, T *out, uint64_t ld, bool vec)
+{
+    const unsigned n_blocks = (x.n_cols + 127) / 128, blk = blockIdx.x % n_blocks, row = blockIdx.x / n_blocks * 32 + threadIdx.x / 8, col = blk * 128 + 16 * (threadIdx.x % 8);
+    if (row >= x.n || col >= x.n_cols) return;
+    const float scale = power(x.scales[(uint64_t)blk * x.ld_scales + row]);
+    const uint4 q = *reinterpret_cast<const uint4 *>(x.values + (uint64_t)row * x.ld + col);
+    float v[16];
+    unpack4(q.x, v), unpack4(q.y, v + 4), unpack4(q.z, v + 8), unpack4(q.w, v + 12);
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] *= scale;
+    T *to = out + (uint64_t)row * ld + col;
+    if (vec && col + 16 <= x.n_cols) store16(to, v);
+    else
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (col + i < x.n_cols) to[i] = from_float<T>(v[i]);
+}
+
+// ---- the matrix's values --------------------------------------------------------------------------------------------
+
+// A block to a CTA, its 64 elements a thread in registers between the search for the largest and the conversion. Thread t has rows
+// 16 i + t / 16 (i = 0..7), columns 8 (t % 16) on. The transposed copy goes through shared memory.
+template <class T>
+__global__ void __launch_bounds__(256) k_block8_set(const T *from, const unsigned *row, const unsigned *col, const unsigned *place, uint8_t *values, uint8_t *scales, uint8_t *values_t,
+                                                    uint8_t *scales_t, unsigned first, unsigned n_rows, unsigned n_cols)
+{
+    __shared__ float largest[8];
+    __shared__ __align__(16) uint8_t tile[128][132];
+    const unsigned b = first + blockIdx.x, r0 = threadIdx.x / 16, c0 = 8 * (threadIdx.x % 16);
+    const T *src = from + (uint64_t)blockIdx.x * 16384 + r0 * 128 + c0;
+    const unsigned rows = min(128u, n_rows - row[b] * 128), cols = min(128u, n_cols - col[b] * 128); // inside the matrix
+    float v[8][8];
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+    {
+        constexpr int per = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < 8; j += per)
+        {
+            const uint4 w = *reinterpret_cast<const uint4 *>(src + i * 16 * 128 + j);
+            const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+            for (int k = 0; k < per; k++)
+            {
+                v[i][j + k] = r0 + 16 * i < rows && c0 + j + k < cols ? to_float(e[k]) : 0.f;
+                most = fmaxf(most, finite_size(v[i][j + k]));
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    if (threadIdx.x % 32 == 0) largest[threadIdx.x / 32] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; i++) most = fmaxf(most, largest[i]);
+    const unsigned scale = scale_of(most);
+    const float inv = inverse(scale);
+    uint8_t *to = values + (uint64_t)b * 16384 + r0 * 128 + c0;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+    {
+        const uint2 q = make_uint2(pack4(v[i], inv), pack4(v[i] + 4, inv));
+        *reinterpret_cast<uint2 *>(to + i * 16 * 128) = q;
+        if (values_t)
+        {
+            unsigned *s = reinterpret_cast<unsigned *>(&tile[r0 + 16 * i][c0]);
+            s[0] = q.x, s[1] = q.y;
+        }
+    }
+    if (threadIdx.x == 0) scales[b] = (uint8_t)scale;
+    if (!values_t) return;
+    const unsigned bt = place[b];
+    if (threadIdx.x == 0) scales_t[bt] = (uint8_t)scale;
+    __syncthreads();
+    // row c of the transposed block: the elements of column c
+    for (unsigned i = threadIdx.x; i < 128 * 32; i += 256)
+    {
+        const unsigned c = i % 128, r = i / 128 * 4; // (consecutive threads, consecutive columns: no conflicts)
+        const unsigned w = tile[r][c] | tile[r + 1][c] << 8 | tile[r + 2][c] << 16 | (unsigned)tile[r + 3][c] << 24;
+        *reinterpret_cast<unsigned *>(values_t + (uint64_t)bt * 16384 + c * 128 + r) = w;
+    }
+}
+
+__global__ void __launch_bounds__(256) k_block8_get(const uint8_t *values, const uint8_t *scales, float *out, unsigned n_blocks)
+{
+    // 16 elements a thread
+    const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 16;
+    const float scale = power(scales[at / 16384]);
+    const uint4 q = *reinterpret_cast<const uint4 *>(values + at);
+    float v[16];
+    unpack4(q.x, v), unpack4(q.y, v + 4), unpack4(q.z, v + 8), unpack4(q.w, v + 12);
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] *= scale;
+    store16(out + at, v);
+}
+
+// ---- products with a few rows ----------------------------------------------------------------------------------------
+
+// Y[t][128 R + r] = sum over the blocks j of block row R of 2^(kA + kX) sum over c of A_j[r][c] X_j[t][c].
+//
+// The matrix is read once and nothing else counts: 16 KB a block straight into registers, as the A operand of m16n8k32 with a warp
+// to 16 rows; X in shared memory, in 8 bits, is the B operand, 8 rows of it a tile. The order of the 128 columns in a sum is free, so a lane takes 16
+// bytes of a row at once (columns 64 h + 16 q on) and its words serve two products. A block's sum is in the products' own units; it is scaled
+// by both powers of two in 32 bits, in two halves, since the product of the two may not be a number although the result is one.
+//
+// A block row is shared by a cluster of CTAs, a contiguous piece of its blocks each, so that all SMs read; the cluster adds up the pieces in
+// order in one another's shared memory: no atomics, no room, the same bits every time.
+constexpr int kFewChunk = 8;                // blocks whose X is in shared memory at once
+constexpr int kFewPitch = 144;              // bytes a row and block: 16-byte reads of 8 lanes in 2 rows meet no conflict
+template <int NT> struct FewShared
+{
+    uint8_t x[kFewChunk][8 * NT][kFewPitch];
+    uint8_t scale[kFewChunk][8 * NT];
+    float part[8 * NT][132];
+};
+
+struct FewArgs
+{
+    Block8Dev a;
+    Rows8Dev held;
+    const void *x;
+    void *y;
+    uint64_t ldx, ldy;
+    unsigned n, n_split;
+    bool vec;
+};
+
+__device__ __forceinline__ uint4 load_once(const uint8_t *p)
+{
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void mma_e4m3(float *c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct Held // X is in 8 bits already
+{
+};
+
+template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_block8_few(const FewArgs args)
+{
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) unsigned char raw[];
+    FewShared<NT> &sh = *reinterpret_cast<FewShared<NT> *>(raw);
+    const cg::cluster_group cluster = cg::this_cluster();
+    const unsigned split = args.n_split, piece = blockIdx.x % split, br = args.a.order[blockIdx.x / split];
+    const unsigned t0 = blockIdx.y * 8 * NT, tokens = min(8u * NT, args.n - t0);
+    const unsigned lo = args.a.ptr[br], len = args.a.ptr[br + 1] - lo;
+    const unsigned j0 = lo + (unsigned)((uint64_t)len * piece / split), j1 = lo + (unsigned)((uint64_t)len * (piece + 1) / split);
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
+
+    const uint8_t *mine = args.a.values + (warp * 16 + g) * 128 + 16 * q;
+    auto load = [&](uint4 *w, unsigned j) {
+        if (j >= j1) return;
+        const uint8_t *p = mine + (uint64_t)j * 16384;
+        w[0] = load_once(p), w[1] = load_once(p + 8 * 128), w[2] = load_once(p + 64), w[3] = load_once(p + 64 + 8 * 128);
+    };
+    float acc[NT][4] = {};
+    auto add = [&](const uint4 *w, unsigned j) {
+        const unsigned slot = (j - j0) % kFewChunk;
+        float c[NT][4] = {};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+            {
+                const uint4 b = *reinterpret_cast<const uint4 *>(&sh.x[slot][8 * nt + g][64 * h + 16 * q]);
+                mma_e4m3(c[nt], w[2 * h].x, w[2 * h + 1].x, w[2 * h].y, w[2 * h + 1].y, b.x, b.y);
+                mma_e4m3(c[nt], w[2 * h].z, w[2 * h + 1].z, w[2 * h].w, w[2 * h + 1].w, b.z, b.w);
+            }
+        const int ka = args.a.scales[j];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+            {
+                const int k = ka + sh.scale[slot][8 * nt + 2 * q + i], half = k / 2; // exponents + 127 each
+                const float f1 = __uint_as_float((unsigned)half << 23), f2 = __uint_as_float((unsigned)(k - half) << 23);
+                acc[nt][i] = __fmaf_rn(c[nt][i] * f1, f2, acc[nt][i]);
+                acc[nt][2 + i] = __fmaf_rn(c[nt][2 + i] * f1, f2, acc[nt][2 + i]);
+            }
+    };
+    uint4 w0[4], w1[4];
+    load(w0, j0);
+    load(w1, j0 + 1);
+    for (unsigned i = threadIdx.x; i < sizeof(sh.x) / 16; i += 256) reinterpret_cast<uint4 *>(sh.x)[i] = make_uint4(0, 0, 0, 0);
+    for (unsigned i = threadIdx.x; i < sizeof(sh.scale); i += 256) (&sh.scale[0][0])[i] = 127;
+    for (unsigned j = j0; j < j1; j += 2)
+    {
+        if ((j - j0) % kFewChunk == 0)
+        {
+            __syncthreads();
+            // 8 lanes to a row's block
+            const unsigned blocks = min((unsigned)kFewChunk, j1 - j), all = blocks * tokens;
+            for (unsigned i = threadIdx.x / 8; i < (all + 3) / 4 * 4; i += 32) // (all four of a warp, for the exchanges)
+            {
+                const unsigned slot = min(i, all - 1) / tokens, t = min(i, all - 1) % tokens, kb = args.a.col[j + slot], lane8 = lane % 8;
+                uint8_t *to = sh.x[slot][t];
+                if constexpr (std::is_same<X, Held>::value)
+                {
+                    const uint64_t row = t0 + t;
+                    *reinterpret_cast<uint4 *>(to + 16 * lane8) = *reinterpret_cast<const uint4 *>(args.held.values + row * args.held.ld + kb * 128 + 16 * lane8);
+                    if (lane8 == 0) sh.scale[slot][t] = args.held.scales[kb * args.held.ld_scales + row];
+                }
+                else
+                {
+                    float v[16];
+                    const bool vec = args.vec && (kb + 1) * 128 <= args.a.n_cols;
+                    load_block(reinterpret_cast<const X *>(args.x) + (uint64_t)(t0 + t) * args.ldx, kb * 128, args.a.n_cols, lane8, vec, v);
+                    const unsigned scale = scale_of(largest_of_8(v));
+                    store_block(v, vec, lane8, scale, to);
+                    if (lane8 == 0) sh.scale[slot][t] = (uint8_t)scale;
+                }
+            }
+            __syncthreads();
+        }
+        add(w0, j);
+        load(w0, j + 2);
+        if (j + 1 < j1) add(w1, j + 1);
+        load(w1, j + 3);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+        {
+            sh.part[8 * nt + 2 * q + i][warp * 16 + g] = acc[nt][i];
+            sh.part[8 * nt + 2 * q + i][warp * 16 + g + 8] = acc[nt][2 + i];
+        }
+    cluster.sync();
+    Y *y = reinterpret_cast<Y *>(args.y);
+    for (unsigned i = threadIdx.x + 256 * piece; i < tokens * 128; i += 256 * split)
+    {
+        const unsigned t = i / 128, r = i % 128;
+        float sum = 0.f;
+        for (unsigned s = 0; s < split; s++) sum += *cluster.map_shared_rank(&sh.part[t][r], s);
+        if (br * 128 + r < args.a.n_rows) y[(uint64_t)(t0 + t) * args.ldy + br * 128 + r] = from_float<Y>(sum);
+    }
+    cluster.sync(); // (its shared memory is read until here)
+}
+
+template <int NT, class X, class Y> cudaError_t few(const FewArgs &args, cudaStream_t st)
+{
+    auto *kernel = k_block8_few<NT, X, Y>;
+    const size_t smem = sizeof(FewShared<NT>);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(args.a.n_block_rows * args.n_split, (args.n + 8 * NT - 1) / (8 * NT));
+    cfg.blockDim = 256;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = args.n_split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+template <class X, class Y> cudaError_t few_by_rows(const FewArgs &args, cudaStream_t st)
+{
+    if (args.n <= 8) return few<1, X, Y>(args, st);
+    if (args.n <= 16) return few<2, X, Y>(args, st);
+    return few<4, X, Y>(args, st);
+}
+} // namespace
+
+cudaError_t launch_rows8_quantize(const Dense &x, unsigned n, const Rows8Dev &out, cudaStream_t st)
+{
+    if (n == 0) return cudaSuccess;
+    return by_type(x.dtype, [&](auto t) {
+        using T = decltype(t);
+        const unsigned grid = (out.n_cols + 511) / 512 * ((n + kQuantRows - 1) / kQuantRows);
+        k_rows8_quantize<T><<<grid, 256, 0, st>>>(reinterpret_cast<const T *>(x.p), x.ld, vectors<T>(x), n, out);
+        return cudaGetLastError();
+    });
+}
+
+cudaError_t launch_rows8_restore(const Rows8Dev &x, const Dense &out, cudaStream_t st)
+{
+    if (x.n == 0) return cudaSuccess;
+    return by_type(out.dtype, [&](auto t) {
+        using T = decltype(t);
+        k_rows8_restore<T><<<(x.n_cols + 127) / 128 * ((x.n + 31) / 32), 256, 0, st>>>(x, reinterpret_cast<T *>(out.p), out.ld, vectors<T>(out));
+        return cudaGetLastError();
+    });
+}
+
+cudaError_t launch_block8_set(const Block8Dev &a, const unsigned *row, const unsigned *place, uint8_t *values, uint8_t *scales, uint8_t *values_t, uint8_t *scales_t, const void *from,
+                              int dtype, unsigned first, unsigned end, cudaStream_t st)
+{
+    if (first >= end) return cudaSuccess;
+    return by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        k_block8_set<T><<<end - first, 256, 0, st>>>(reinterpret_cast<const T *>(from), row, a.col, place, values, scales, values_t, scales_t, first, a.n_rows, a.n_cols);
+        return cudaGetLastError();
+    });
+}
+
+cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st)
+{
+    if (a.n_blocks == 0) return cudaSuccess;
+    k_block8_get<<<a.n_blocks * 4, 256, 0, st>>>(a.values, a.scales, out, a.n_blocks);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, cudaStream_t st)
+{
+    if (n == 0) return cudaSuccess;
+    FewArgs args = {};
+    args.a = a;
+    args.n = n;
+    args.y = y.p;
+    args.ldy = y.ld;
+    const unsigned tiles = (n + 31) / 32;
+    args.n_split = 1; // two CTAs fit an SM
+    while (args.n_split < 8 && args.n_split * 2 <= a.longest && a.n_block_rows * tiles * args.n_split < 2u * sm_count) args.n_split *= 2;
+    return by_type(y.dtype, [&](auto ty) {
+        using Y = decltype(ty);
+        if (held)
+        {
+            args.held = *held;
+            return few_by_rows<Held, Y>(args, st);
+        }
+        args.x = x->p;
+        args.ldx = x->ld;
+        return by_type(x->dtype, [&](auto tx) {
+            using X = decltype(tx);
+            args.vec = vectors<X>(*x);
+            return few_by_rows<X, Y>(args, st);
+        });
+    });
+}
+} // namespace asp

@@ -41,7 +41,9 @@ typedef enum asp_dtype
     ASP_U32 = 2,
     ASP_U64 = 3,
     ASP_F32 = 4,
-    ASP_F64 = 5
+    ASP_F64 = 5,
+    ASP_F16 = 6, /* operands of asp_b200_block8.h, as ASP_BF16: not for format arrays */
+    ASP_BF16 = 7
 } asp_dtype;
 
 /* closed forms that stand in for a metadata array (arr_optimization.hpp:12-81). The
@@ -396,6 +398,8 @@ asp_status asp_time(asp_ctx *ctx, asp_plan *const *plans, int n_plans, int warmu
  * (part_execute_code_builder + execute_binary, executor.cc:6-260). */
 asp_status asp_search_gpu(asp_ctx *ctx, const void *matrix, const void *options, void **result);
 
+/* Waits for the context's stream. ASP_ERR_TIMEOUT: a kernel of asp_b200_block8.h gave up one of its bounded waits; its results
+ * are not complete. */
 asp_status asp_synchronize(asp_ctx *ctx);
 const char *asp_status_str(asp_status s);
 /* text of the last CUDA error seen by this thread ("" if none) */
