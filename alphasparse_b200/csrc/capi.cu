@@ -515,6 +515,8 @@ asp_status asp_ctx_create(int device, asp_ctx **out)
         e = cudaStreamCreateWithFlags(&c->aux[i], cudaStreamNonBlocking);
         if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->ev_join[i], cudaEventDisableTiming);
     }
+    if (e == cudaSuccess) e = cudaHostAlloc((void **)&c->fault, sizeof(*c->fault), cudaHostAllocPortable | cudaHostAllocMapped);
+    if (e == cudaSuccess) *c->fault = 0;
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&c->max_smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
     if (e != cudaSuccess)
@@ -534,6 +536,7 @@ void asp_ctx_destroy(asp_ctx *c)
     c->stager.release();
     if (c->x) cudaFree(c->x);
     if (c->y) cudaFree(c->y);
+    if (c->fault) cudaFreeHost(c->fault);
     if (c->ev0) cudaEventDestroy(c->ev0);
     if (c->ev1) cudaEventDestroy(c->ev1);
     if (c->ev_fork) cudaEventDestroy(c->ev_fork);
@@ -559,7 +562,10 @@ asp_status asp_synchronize(asp_ctx *ctx)
     if (!ctx) return fail(ASP_ERR_INVALID_ARG, "ctx is NULL");
     ASP_ON_DEVICE(ctx);
     ASP_CUDA(cudaStreamSynchronize(ctx->stream));
-    return ASP_OK;
+    volatile unsigned *fault = ctx->fault;
+    if (!*fault) return ASP_OK;
+    *fault = 0;
+    return fail(ASP_ERR_TIMEOUT, "a kernel gave up waiting for its own copies or products");
 }
 
 } // extern "C"

@@ -39,7 +39,7 @@ struct asp_block8
     asp::host::Block8Pattern pattern;
     asp::Block8Dev side[2] = {};
     const unsigned *row = nullptr, *place = nullptr;
-    uint8_t *values[2] = {nullptr, nullptr}, *scales[2] = {nullptr, nullptr};
+    asp::Block8Set set[2] = {};
     bool transposed = false;
     size_t bytes = 0;
 };
@@ -94,11 +94,12 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
         return r;
     };
     const int sides = m->transposed ? 2 : 1;
-    Piece values[2], scales[2], ptr[2], col[2], order[2];
+    Piece values[2], scales[2], scale_rows[2], ptr[2], col[2], order[2];
     for (int s = 0; s < sides; s++)
     {
         values[s] = take(n * kBlock8 * kBlock8);
         scales[s] = take(n);
+        scale_rows[s] = take(n * 512);
         ptr[s] = take(p.side[s].ptr.size() * 4);
         col[s] = take(n * 4);
         order[s] = take(p.side[s].order.size() * 4);
@@ -125,15 +126,17 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
     {
         const asp::host::Block8Side &h = p.side[s];
         asp::Block8Dev &d = m->side[s];
-        d.values = m->values[s] = base + values[s].at;
-        d.scales = m->scales[s] = base + scales[s].at;
+        d.values = m->set[s].values = base + values[s].at;
+        d.scales = m->set[s].scales = base + scales[s].at;
+        d.scale_rows = m->set[s].scale_rows = base + scale_rows[s].at;
         d.ptr = send(ptr[s], h.ptr.data());
         d.col = send(col[s], h.col.data());
         d.order = send(order[s], h.order.data());
         d.n_block_rows = h.rows(), d.n_blocks = (unsigned)n, d.longest = h.longest;
         d.n_rows = (unsigned)(s ? p.n_cols : p.n_rows), d.n_cols = (unsigned)(s ? p.n_rows : p.n_cols);
-        e = cudaMemsetAsync(m->values[s], 0, values[s].bytes, ctx->stream);
-        if (e == cudaSuccess) e = cudaMemsetAsync(m->scales[s], 127, scales[s].bytes, ctx->stream);
+        e = cudaMemsetAsync(base + values[s].at, 0, values[s].bytes, ctx->stream);
+        if (e == cudaSuccess) e = cudaMemsetAsync(base + scales[s].at, 127, scales[s].bytes, ctx->stream);
+        if (e == cudaSuccess) e = cudaMemsetAsync(base + scale_rows[s].at, 127, scale_rows[s].bytes, ctx->stream);
         if (e != cudaSuccess) return cuda_fail(e, "clearing the values");
     }
     m->row = send(row, rows.data());
@@ -189,12 +192,12 @@ asp_status asp_rows8_create(asp_ctx *ctx, uint64_t max_rows, uint64_t n_cols, as
         std::unique_ptr<asp_rows8> r(new asp_rows8());
         r->max_rows = max_rows;
         r->dev.ld = up(n_cols, kBlock8);
-        r->dev.ld_scales = up(max_rows, 32);
+        r->dev.pieces = (unsigned)(up(max_rows, kBlock8) / kBlock8);
         r->dev.n_cols = (unsigned)n_cols;
         const uint64_t values = up(max_rows * r->dev.ld, 1024);
         ASP_ON_DEVICE(ctx);
         r->room.device = ctx->device;
-        const cudaError_t e = asp::device_alloc(ctx->device, values + r->dev.ld / kBlock8 * r->dev.ld_scales, &r->room.base, &r->room.got);
+        const cudaError_t e = asp::device_alloc(ctx->device, values + up(r->dev.ld, 4 * kBlock8) / (4 * kBlock8) * r->dev.pieces * 512, &r->room.base, &r->room.got);
         if (e != cudaSuccess)
         {
             r->room.base = nullptr;
@@ -278,7 +281,7 @@ asp_status asp_block8_from_matrix(asp_ctx *ctx, const void *matrix, int transpos
             asp::host::block_values(h, m->pattern, b, end, values.data());
             e = ctx->stager.to_device(room.base, values.data(), (end - b) * kBlock8 * kBlock8 * 4, ctx->stream);
             if (e == cudaSuccess)
-                e = asp::launch_block8_set(m->side[0], m->row, m->place, m->values[0], m->scales[0], m->values[1], m->scales[1], room.base, ASP_F32, (unsigned)b, (unsigned)end, ctx->stream);
+                e = asp::launch_block8_set(m->side[0], m->row, m->place, m->set, room.base, ASP_F32, (unsigned)b, (unsigned)end, ctx->stream);
         }
         const cudaError_t done = cudaStreamSynchronize(ctx->stream);
         if (e == cudaSuccess) e = done;
@@ -308,7 +311,7 @@ asp_status asp_block8_set_values(asp_ctx *ctx, asp_block8 *m, const void *d_valu
     if ((!d_values && m->pattern.blocks()) || (uintptr_t)d_values % 16) return fail(ASP_ERR_INVALID_ARG, "values are NULL or not on a 16-byte boundary");
     ASP_TRY(same_device(ctx, m->room));
     ASP_ON_DEVICE(ctx);
-    return launched(asp::launch_block8_set(m->side[0], m->row, m->place, m->values[0], m->scales[0], m->values[1], m->scales[1], d_values, dtype, 0, (unsigned)m->pattern.blocks(), ctx->stream));
+    return launched(asp::launch_block8_set(m->side[0], m->row, m->place, m->set, d_values, dtype, 0, (unsigned)m->pattern.blocks(), ctx->stream));
 }
 
 asp_status asp_block8_get_values(asp_ctx *ctx, const asp_block8 *m, float *d_values)
@@ -345,7 +348,8 @@ asp_status asp_block8_product(asp_ctx *ctx, const asp_block8 *m, int transposed,
     ASP_TRY(same_device(ctx, m->room));
     ASP_TRY(same_device(ctx, x->room));
     ASP_ON_DEVICE(ctx);
-    return launched(asp::launch_block8_few(*a, nullptr, &x->dev, x->dev.n, y, ctx->sm_count, ctx->stream));
+    if (x->dev.n <= ASP_BLOCK8_APPLY_ROWS) return launched(asp::launch_block8_few(*a, nullptr, &x->dev, x->dev.n, y, ctx->sm_count, ctx->stream));
+    return launched(asp::launch_block8_product(*a, x->dev, y, ctx->sm_count, ctx->fault, ctx->stream));
 }
 
 asp_status asp_block8_gradient(asp_ctx *ctx, const asp_block8 *m, const asp_rows8 *x, const void *d_dy, int dtype, uint64_t ld, float *d_out, int accumulate)

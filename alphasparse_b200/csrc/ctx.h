@@ -75,6 +75,7 @@ struct asp_ctx
     cudaStream_t h2d = nullptr, d2h = nullptr;
     std::vector<cudaEvent_t> pipe_events;
     asp::Stager stager;
+    unsigned *fault = nullptr; // page-locked: set by a kernel that gives up a bounded wait, read by asp_synchronize
 };
 
 #endif

@@ -25,12 +25,12 @@ template <class T> bool vectors(const Dense &x) { return ((uintptr_t)x.p & 15) =
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
 // 32 rows x 512 columns to a CTA of 8 warps: a warp takes a row's four blocks at once, 8 lanes and 16 elements a lane each, so that an
-// element is read once and its block's largest is known after three exchanges. Bounded by memory. The scales of a block column
-// are collected so that they leave as 32 bytes in a row instead of one by one.
+// element is read once and its block's largest is known after three exchanges. Bounded by memory. A row's four scales leave as a
+// word.
 constexpr int kQuantRows = 32;
 template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const T *x, uint64_t ld, bool vec, unsigned n, Rows8Dev out)
 {
-    __shared__ uint8_t scales[4][kQuantRows];
+    __shared__ __align__(4) uint8_t scales[kQuantRows][4];
     const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (out.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
     const unsigned blk0 = blockIdx.x % fours * 4, blk = blk0 + lane / 8, row0 = blockIdx.x / fours * kQuantRows;
 #pragma unroll
@@ -45,11 +45,12 @@ template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const
         if (!there) continue;
         const unsigned scale = scale_of(most);
         store_block(v, together, lane8, scale, out.values + (uint64_t)row * out.ld + blk * 128);
-        if (lane8 == 0) scales[lane / 8][i * 8 + warp] = (uint8_t)scale;
+        if (lane8 == 0) scales[i * 8 + warp][lane / 8] = (uint8_t)scale;
     }
     __syncthreads();
-    const unsigned b = threadIdx.x / kQuantRows, r = threadIdx.x % kQuantRows;
-    if (b < 4 && blk0 + b < n_blocks && row0 + r < n) out.scales[(uint64_t)(blk0 + b) * out.ld_scales + row0 + r] = scales[b][r];
+    const unsigned r = threadIdx.x;
+    if (r < kQuantRows && row0 + r < n) // the four blocks' bytes are a word (those behind the last block are not used)
+        *reinterpret_cast<unsigned *>(out.scales + scale_at(out, row0 + r, blk0)) = *reinterpret_cast<const unsigned *>(scales[r]);
 }
 
 // 16 columns to a thread, a block of 128 columns and 32 rows to a CTA
@@ -57,7 +58,7 @@ template <class T> __global__ void __launch_bounds__(256) k_rows8_restore(Rows8D
 {
     const unsigned n_blocks = (x.n_cols + 127) / 128, blk = blockIdx.x % n_blocks, row = blockIdx.x / n_blocks * 32 + threadIdx.x / 8, col = blk * 128 + 16 * (threadIdx.x % 8);
     if (row >= x.n || col >= x.n_cols) return;
-    const float scale = power(x.scales[(uint64_t)blk * x.ld_scales + row]);
+    const float scale = power(x.scales[scale_at(x, row, blk)]);
     const uint4 q = *reinterpret_cast<const uint4 *>(x.values + (uint64_t)row * x.ld + col);
     float v[16];
     unpack4(q.x, v), unpack4(q.y, v + 4), unpack4(q.z, v + 8), unpack4(q.w, v + 12);
@@ -75,9 +76,14 @@ template <class T> __global__ void __launch_bounds__(256) k_rows8_restore(Rows8D
 
 // A block to a CTA, its 64 elements a thread in registers between the search for the largest and the conversion. Thread t has rows
 // 16 i + t / 16 (i = 0..7), columns 8 (t % 16) on. The transposed copy goes through shared memory.
+__device__ __forceinline__ void put_scale(const Block8Set &to, unsigned block, unsigned scale)
+{
+    if (threadIdx.x == 0) to.scales[block] = (uint8_t)scale;
+    if (threadIdx.x < 128) reinterpret_cast<unsigned *>(to.scale_rows)[(uint64_t)block * 128 + threadIdx.x] = scale * 0x01010101u;
+}
 template <class T>
-__global__ void __launch_bounds__(256) k_block8_set(const T *from, const unsigned *row, const unsigned *col, const unsigned *place, uint8_t *values, uint8_t *scales, uint8_t *values_t,
-                                                    uint8_t *scales_t, unsigned first, unsigned n_rows, unsigned n_cols)
+__global__ void __launch_bounds__(256) k_block8_set(const T *from, const unsigned *row, const unsigned *col, const unsigned *place, Block8Set a, Block8Set t, unsigned first, unsigned n_rows,
+                                                    unsigned n_cols)
 {
     __shared__ float largest[8];
     __shared__ __align__(16) uint8_t tile[128][132];
@@ -111,29 +117,29 @@ __global__ void __launch_bounds__(256) k_block8_set(const T *from, const unsigne
     for (int i = 0; i < 8; i++) most = fmaxf(most, largest[i]);
     const unsigned scale = scale_of(most);
     const float inv = inverse(scale);
-    uint8_t *to = values + (uint64_t)b * 16384 + r0 * 128 + c0;
+    uint8_t *to = a.values + (uint64_t)b * 16384 + r0 * 128 + c0;
 #pragma unroll
     for (int i = 0; i < 8; i++)
     {
         const uint2 q = make_uint2(pack4(v[i], inv), pack4(v[i] + 4, inv));
         *reinterpret_cast<uint2 *>(to + i * 16 * 128) = q;
-        if (values_t)
+        if (t.values)
         {
             unsigned *s = reinterpret_cast<unsigned *>(&tile[r0 + 16 * i][c0]);
             s[0] = q.x, s[1] = q.y;
         }
     }
-    if (threadIdx.x == 0) scales[b] = (uint8_t)scale;
-    if (!values_t) return;
+    put_scale(a, b, scale);
+    if (!t.values) return;
     const unsigned bt = place[b];
-    if (threadIdx.x == 0) scales_t[bt] = (uint8_t)scale;
+    put_scale(t, bt, scale);
     __syncthreads();
     // row c of the transposed block: the elements of column c
     for (unsigned i = threadIdx.x; i < 128 * 32; i += 256)
     {
         const unsigned c = i % 128, r = i / 128 * 4; // (consecutive threads, consecutive columns: no conflicts)
         const unsigned w = tile[r][c] | tile[r + 1][c] << 8 | tile[r + 2][c] << 16 | (unsigned)tile[r + 3][c] << 24;
-        *reinterpret_cast<unsigned *>(values_t + (uint64_t)bt * 16384 + c * 128 + r) = w;
+        *reinterpret_cast<unsigned *>(t.values + (uint64_t)bt * 16384 + c * 128 + r) = w;
     }
 }
 
@@ -261,7 +267,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
                 {
                     const uint64_t row = t0 + t;
                     *reinterpret_cast<uint4 *>(to + 16 * lane8) = *reinterpret_cast<const uint4 *>(args.held.values + row * args.held.ld + kb * 128 + 16 * lane8);
-                    if (lane8 == 0) sh.scale[slot][t] = args.held.scales[kb * args.held.ld_scales + row];
+                    if (lane8 == 0) sh.scale[slot][t] = args.held.scales[scale_at(args.held, row, kb)];
                 }
                 else
                 {
@@ -348,13 +354,12 @@ cudaError_t launch_rows8_restore(const Rows8Dev &x, const Dense &out, cudaStream
     });
 }
 
-cudaError_t launch_block8_set(const Block8Dev &a, const unsigned *row, const unsigned *place, uint8_t *values, uint8_t *scales, uint8_t *values_t, uint8_t *scales_t, const void *from,
-                              int dtype, unsigned first, unsigned end, cudaStream_t st)
+cudaError_t launch_block8_set(const Block8Dev &a, const unsigned *row, const unsigned *place, const Block8Set to[2], const void *from, int dtype, unsigned first, unsigned end, cudaStream_t st)
 {
     if (first >= end) return cudaSuccess;
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        k_block8_set<T><<<end - first, 256, 0, st>>>(reinterpret_cast<const T *>(from), row, a.col, place, values, scales, values_t, scales_t, first, a.n_rows, a.n_cols);
+        k_block8_set<T><<<end - first, 256, 0, st>>>(reinterpret_cast<const T *>(from), row, a.col, place, to[0], to[1], first, a.n_rows, a.n_cols);
         return cudaGetLastError();
     });
 }

@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256) k_block8_gradient(Block8Dev a, const unsi
             if (t < x.n)
             {
                 unpack4(*reinterpret_cast<const unsigned *>(x.values + t * x.ld + cb * 128 + c), v);
-                const float scale = power(x.scales[cb * x.ld_scales + t]);
+                const float scale = power(x.scales[scale_at(x, t, cb)]);
                 for (int k = 0; k < 4; k++) v[k] *= scale;
             }
             for (int k = 0; k < 4; k++) sx[i / 32][c + k] = v[k];

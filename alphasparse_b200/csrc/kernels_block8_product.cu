@@ -1,0 +1,299 @@
+// Products of block-sparse 8-bit matrices with many rows in 8 bits (asp_block8_product).
+#include <math.h>
+
+#include <algorithm>
+
+#include "../../include/asp_b200.h"
+#include "block8.h"
+#include "block8_device.h"
+#include "tcgen05.h"
+#include "tensor_map.h"
+
+namespace asp
+{
+namespace
+{
+using namespace block8;
+
+// Y[t][128 R + r] = sum over the blocks j of block row R of 2^(kA_j) sum over c of A_j[r][c] * 2^(kX_{t, c_j}) X_{t, c_j}[c].
+//
+// A tile is 128 rows of A by up to 192 rows of X: D[128][192] in tensor memory, a block of A (16 KB) and the same 128 columns of X (24 KB) a
+// step, four tcgen05.mma of 32 columns each. The powers of two go into the products as their scales (a byte per row of the block and per row of X), so sums
+// over blocks of different scales stay in tensor memory, in 32 bits, from the first block to the last. A's rows are the
+// rows of D because a block is 128 rows of A whatever the pattern, while X can be cut anywhere; 192 since two tiles' sums (384
+// columns) and the scales (24) then share the 512 columns, so that a tile is stored under the next one's products, and whole 64s since the
+// scales of X begin at every second column.
+//
+// A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 9 store.
+constexpr unsigned kMostRows = 192;
+constexpr unsigned kStages = 8; // at most
+constexpr unsigned kScaleBytes = 512 + 1024;
+constexpr unsigned kRoom = 221 * 1024; // of shared memory for stages
+constexpr unsigned kThreads = 320;
+
+struct ProductArgs
+{
+    Block8Dev a;
+    Rows8Dev x;
+    void *y;
+    uint64_t ldy;
+    unsigned tile;   // rows of X a tile, a multiple of 64
+    unsigned tiles_x, group;
+    unsigned n_tiles;
+    unsigned stages, stage_bytes;
+    bool pairs;      // two 16-bit elements of y at a time
+    unsigned *fault;
+};
+
+struct Shared
+{
+    uint64_t full[kStages], empty[kStages], done[2], taken[2];
+    unsigned tensor, gave_up;
+};
+
+// The steps of a CTA, in order: the blocks of its tiles. A tile is given by its place among tiles in groups of `group` block rows times all tiles of X, so
+// that the tiles that run at the same time share blocks of A and rows of X in L2.
+struct Steps
+{
+    const ProductArgs &p;
+    unsigned tile, j = 0, end = 0, row = 0, t0 = 0;
+    __device__ __forceinline__ Steps(const ProductArgs &args, unsigned first) : p(args), tile(first) { locate(); }
+    __device__ __forceinline__ bool valid() const { return tile < p.n_tiles; }
+    __device__ __forceinline__ void locate()
+    {
+        if (!valid()) return;
+        const unsigned per = p.group * p.tiles_x, g = tile / per, in = tile % per, rows = min(p.group, p.a.n_block_rows - g * p.group);
+        row = p.a.order[g * p.group + in % rows];
+        t0 = in / rows * p.tile;
+        j = p.a.ptr[row], end = p.a.ptr[row + 1];
+    }
+    __device__ __forceinline__ void next_tile()
+    {
+        tile += gridDim.x;
+        locate();
+    }
+};
+
+template <class Y> __device__ __forceinline__ void store_columns(const float *v, const ProductArgs &p, unsigned row0, unsigned lane, unsigned t0, unsigned limit)
+{
+    Y *y = reinterpret_cast<Y *>(p.y);
+    const unsigned row = row0 + lane;
+    if constexpr (sizeof(Y) == 2)
+    {
+        if (p.pairs)
+        {
+            // lanes 2 i and 2 i + 1 exchange, so that each has two rows of one column: 4 bytes
+            const bool odd = lane & 1;
+            Y *to = y + (uint64_t)(t0 + odd) * p.ldy + (row & ~1u);
+            const bool both = (row & ~1u) + 1 < p.a.n_rows, one = (row & ~1u) < p.a.n_rows;
+#pragma unroll
+            for (int c = 0; c < 32; c += 2)
+            {
+                const float got = __shfl_xor_sync(~0u, odd ? v[c] : v[c + 1], 1);
+                const Y lo = from_float<Y>(odd ? got : v[c]), hi = from_float<Y>(odd ? v[c + 1] : got);
+                if (t0 + c + odd < limit)
+                {
+                    if (both)
+                    {
+                        Y two[2] = {lo, hi};
+                        *reinterpret_cast<unsigned *>(to) = *reinterpret_cast<unsigned *>(two);
+                    }
+                    else if (one) *to = lo;
+                }
+                to += 2 * p.ldy;
+            }
+            return;
+        }
+    }
+    if (row >= p.a.n_rows) return;
+#pragma unroll
+    for (int c = 0; c < 32; c++)
+        if (t0 + c < limit) y[(uint64_t)(t0 + c) * p.ldy + row] = from_float<Y>(v[c]);
+}
+
+template <class Y>
+__global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ ProductArgs p)
+{
+    extern __shared__ unsigned char raw[];
+    __shared__ Shared sh;
+    unsigned char *stages = raw + (1024 - tc::shared_address(raw) % 1024) % 1024;
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0)
+    {
+        for (unsigned i = 0; i < p.stages; i++)
+        {
+            tc::barrier_init(&sh.full[i], 1);
+            tc::barrier_init(&sh.empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++)
+        {
+            tc::barrier_init(&sh.done[i], 1);
+            tc::barrier_init(&sh.taken[i], 8);
+        }
+        sh.gave_up = 0;
+        tc::fence_barrier_init();
+    }
+    if (warp == 1) tc::tensor_alloc(&sh.tensor, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const unsigned tensor = sh.tensor;
+    const unsigned x_bytes = p.tile * 128;
+
+    if (warp == 0)
+    {
+        if (lane == 0)
+        {
+            tc::prefetch_map(&map_a), tc::prefetch_map(&map_x);
+            unsigned s = 0, phase = 0;
+            for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
+                for (; at.j < at.end; at.j++)
+                {
+                    const unsigned col = p.a.col[at.j];
+                    if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
+                    unsigned char *to = stages + s * p.stage_bytes;
+                    // scales of X: the pieces of 128 rows that have rows of the tile
+                    const unsigned piece = at.t0 / 128, pieces = (min(at.t0 + p.tile, p.x.n) + 127) / 128 - piece;
+                    tc::barrier_expect(&sh.full[s], 16384 + x_bytes + 512 + pieces * 512);
+                    tc::copy_tile(to, &map_a, 0, (int)(at.j * 128), &sh.full[s]);
+                    tc::copy_tile(to + 16384, &map_x, (int)(col * 128), (int)at.t0, &sh.full[s]);
+                    tc::copy_bytes(to + 16384 + x_bytes, p.a.scale_rows + (uint64_t)at.j * 512, 512, &sh.full[s]);
+                    tc::copy_bytes(to + 16384 + x_bytes + 512, p.x.scales + ((uint64_t)(col / 4) * p.x.pieces + piece) * 512, pieces * 512, &sh.full[s]);
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+        }
+    }
+    else if (warp == 1)
+    {
+        if (lane == 0)
+        {
+            unsigned s = 0, phase = 0, b = 0, b_phase = 0, turn = 0;
+            for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
+            {
+                if (at.j == at.end) continue;
+                if (!tc::barrier_wait(&sh.taken[b], b_phase ^ 1, &sh.gave_up)) goto end;
+                tc::fence_after();
+                const unsigned d = tensor + b * kMostRows, shift = at.t0 % 128 / 32; // (of the first row among its piece's columns)
+                bool add = false;
+                for (; at.j < at.end; at.j++)
+                {
+                    const unsigned shape = tc::scaled_e4m3(p.tile, p.a.col[at.j] % 4);
+                    if (!tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
+                    tc::fence_after();
+                    const unsigned a = tc::shared_address(stages + s * p.stage_bytes), x = a + 16384, scales = x + x_bytes;
+                    const unsigned sa = tensor + 2 * kMostRows + turn * 4, sx = tensor + 2 * kMostRows + 8 + turn * 8;
+                    tc::copy_scales(sa, tc::scale_rows(scales));
+                    tc::copy_scales(sx, tc::scale_rows(scales + 512));
+                    if (shift + p.tile / 32 > 4) tc::copy_scales(sx + 4, tc::scale_rows(scales + 1024));
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                    {
+                        tc::mma_scaled(d, tc::rows_k_major(a + 32 * k), tc::rows_k_major(x + 32 * k), shape, sa, sx + shift, add);
+                        add = true;
+                    }
+                    tc::commit(&sh.empty[s]);
+                    turn ^= 1;
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+                tc::commit(&sh.done[b]);
+                b ^= 1;
+                if (b == 0) b_phase ^= 1;
+            }
+        }
+    }
+    else
+    {
+        unsigned b = 0, b_phase = 0;
+        const unsigned quarter = warp % 4, first = (warp - 2) / 4 * 32; // two warps to a quarter of D's lanes, every second 32 columns each
+        for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
+        {
+            const unsigned row0 = at.row * 128 + quarter * 32, limit = min(p.x.n, at.t0 + p.tile);
+            float v[32];
+            if (at.j == at.end)
+            {
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = 0.f;
+                for (unsigned c = first; c < p.tile; c += 64) store_columns<Y>(v, p, row0, lane, at.t0 + c, limit);
+                continue;
+            }
+            if (!tc::barrier_wait(&sh.done[b], b_phase, &sh.gave_up)) break;
+            tc::fence_after();
+            for (unsigned c = first; c < p.tile; c += 64)
+            {
+                tc::tensor_load32(tensor + b * kMostRows + c + (quarter * 32 << 16), v);
+                store_columns<Y>(v, p, row0, lane, at.t0 + c, limit);
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::barrier_arrive(&sh.taken[b]);
+            b ^= 1;
+            if (b == 0) b_phase ^= 1;
+        }
+    }
+end:
+    __syncwarp();
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (sh.gave_up)
+    {
+        // copies and products in flight end by themselves; their memory is kept until then
+        const uint64_t since = tc::now_ns();
+        while (tc::now_ns() - since < 10000000ull) __nanosleep(1000);
+        if (threadIdx.x == 0 && p.fault) *reinterpret_cast<volatile unsigned *>(p.fault) = 1;
+    }
+    if (warp == 1) tc::tensor_free(tensor, 512);
+}
+
+// Rows of X a tile. The steps of a tile take as long as their products (2 clocks a row of X) or their copies do (some 50 bytes a clock and SM); a tile
+// costs some 2000 clocks beside its steps. Every size is looked at, for the waves that its tiles make of the SMs.
+unsigned tile_rows(const Block8Dev &a, unsigned n, int sm_count)
+{
+    const double steps = (double)a.n_blocks / a.n_block_rows;
+    unsigned best = kMostRows;
+    double least = 0;
+    for (unsigned t = kMostRows; t >= 64; t -= 64)
+    {
+        const uint64_t tiles = (uint64_t)a.n_block_rows * ((n + t - 1) / t), waves = (tiles + sm_count - 1) / sm_count;
+        const double cost = waves * (2000.0 + steps * std::max(2.0 * t, (16384.0 + 128.0 * t) / 50.0));
+        if (t == kMostRows || cost < least) best = t, least = cost;
+    }
+    return best;
+}
+
+template <class Y> cudaError_t product(const CUtensorMap &map_a, const CUtensorMap &map_x, const ProductArgs &p, int sm_count, cudaStream_t st)
+{
+    const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(k_block8_product<Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    k_block8_product<Y><<<std::min<unsigned>(p.n_tiles, (unsigned)sm_count), kThreads, smem, st>>>(map_a, map_x, p);
+    return cudaGetLastError();
+}
+} // namespace
+
+cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st)
+{
+    if (x.n == 0) return cudaSuccess;
+    ProductArgs p = {};
+    p.a = a, p.x = x, p.y = y.p, p.ldy = y.ld, p.fault = fault;
+    p.tile = tile_rows(a, x.n, sm_count);
+    p.tiles_x = (x.n + p.tile - 1) / p.tile;
+    const uint64_t tiles = (uint64_t)a.n_block_rows * p.tiles_x;
+    if (tiles > 0xf0000000u) return cudaErrorInvalidValue; // (2^38 rows of blocks' results and more)
+    p.n_tiles = (unsigned)tiles;
+    // block rows that run together: as many bytes of A as of X
+    const double side = (double)p.tile * x.ld / std::max(1.0, 16384.0 * a.n_blocks / a.n_block_rows);
+    p.group = std::min<unsigned>(a.n_block_rows, std::max(1u, (unsigned)sqrt(sm_count * side)));
+    p.stage_bytes = (16384 + p.tile * 128 + kScaleBytes + 1023) / 1024 * 1024;
+    p.stages = std::min(kStages, kRoom / p.stage_bytes);
+    p.pairs = y.dtype != ASP_F32 && ((uintptr_t)y.p & 3) == 0 && y.ld % 2 == 0;
+    CUtensorMap map_a, map_x;
+    // (a matrix without blocks has nothing to copy: any map does)
+    cudaError_t e = byte_map(&map_a, a.values, 128, (uint64_t)std::max(1u, a.n_blocks) * 128, 128, 128);
+    if (e == cudaSuccess) e = byte_map(&map_x, x.values, x.ld, x.n, x.ld, p.tile);
+    if (e != cudaSuccess) return e;
+    if (y.dtype == ASP_F32) return product<float>(map_a, map_x, p, sm_count, st);
+    if (y.dtype == ASP_F16) return product<__half>(map_a, map_x, p, sm_count, st);
+    return product<__nv_bfloat16>(map_a, map_x, p, sm_count, st);
+}
+} // namespace asp

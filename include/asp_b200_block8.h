@@ -38,7 +38,7 @@ typedef struct asp_rows8 asp_rows8;
 
 /* ---- rows in 8 bits ---- */
 
-/* Room for up to max_rows rows of n_cols columns (a byte each, rounded up to 128, and a byte per row and 128 columns). */
+/* Room for up to max_rows rows of n_cols columns (a byte each, and a byte for each row and 128 columns; rows in whole 128s, columns in whole 512s at most). */
 asp_status asp_rows8_create(asp_ctx *ctx, uint64_t max_rows, uint64_t n_cols, asp_rows8 **out);
 void asp_rows8_destroy(asp_rows8 *rows);
 /* X (n rows, ASP_F32 | ASP_F16 | ASP_BF16) to 8 bits; the handle then holds n rows. Rows behind them are left as they were. */
