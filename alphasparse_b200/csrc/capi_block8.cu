@@ -38,7 +38,7 @@ struct asp_block8
     Room room;
     asp::host::Block8Pattern pattern;
     asp::Block8Dev side[2] = {};
-    const unsigned *row = nullptr, *place = nullptr;
+    const unsigned *row = nullptr, *place = nullptr, *pairs = nullptr;
     asp::Block8Set set[2] = {};
     bool transposed = false;
     size_t bytes = 0;
@@ -104,7 +104,7 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
         col[s] = take(n * 4);
         order[s] = take(p.side[s].order.size() * 4);
     }
-    const Piece row = take(n * 4), place = take(n * 4);
+    const Piece row = take(n * 4), place = take(n * 4), pairs = take(p.pairs.size() * 4);
     std::vector<uint32_t> rows(n);
     for (uint32_t r = 0; r < p.side[0].rows(); r++) std::fill(rows.begin() + p.side[0].ptr[r], rows.begin() + p.side[0].ptr[r + 1], r);
     ASP_ON_DEVICE(ctx);
@@ -141,6 +141,7 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
     }
     m->row = send(row, rows.data());
     m->place = send(place, p.place.data());
+    m->pairs = send(pairs, p.pairs.data());
     e = ctx->stager.to_device(m->room.base, segments, ctx->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) return cuda_fail(e, "upload of the pattern");
@@ -364,7 +365,7 @@ asp_status asp_block8_gradient(asp_ctx *ctx, const asp_block8 *m, const asp_rows
     ASP_TRY(same_device(ctx, m->room));
     ASP_TRY(same_device(ctx, x->room));
     ASP_ON_DEVICE(ctx);
-    return launched(asp::launch_block8_gradient(m->side[0], m->row, x->dev, dy, d_out, accumulate != 0, ctx->sm_count, ctx->stream));
+    return launched(asp::launch_block8_gradient(m->side[0], m->row, m->pairs, (unsigned)m->pattern.pairs.size(), x->dev, dy, d_out, accumulate != 0, ctx->sm_count, ctx->fault, ctx->stream));
 }
 
 } // extern "C"

@@ -64,6 +64,8 @@ asp_status make_pattern(u64 n_rows, u64 n_cols, const int64_t *block_ptr, const 
             out.place[j] = next[a.col[j]]++;
             t.col[out.place[j]] = r;
         }
+    for (u64 r = 0; r < nr; r++)
+        for (u32 j = a.ptr[r]; j < a.ptr[r + 1]; j += 2) out.pairs.push_back(j | (j + 1 < a.ptr[r + 1] ? 1u << 31 : 0u));
     finish(a);
     finish(t);
     return ASP_OK;

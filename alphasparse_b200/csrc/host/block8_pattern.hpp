@@ -29,6 +29,7 @@ struct Block8Pattern
     u64 n_rows = 0, n_cols = 0;
     Block8Side side[2];      // of A, of A^T
     std::vector<u32> place;  // where block i of A lies among the blocks of A^T
+    std::vector<u32> pairs;  // blocks of A two by two: the first, and in bit 31 whether the next one is of the same block row and belongs to it
     u64 blocks() const { return side[0].col.size(); }
 };
 

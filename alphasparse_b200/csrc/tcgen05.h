@@ -101,6 +101,16 @@ __device__ __forceinline__ void commit(uint64_t *b)
 // Rows of 128 bytes of k, in the copies' 128-byte swizzle: groups of 8 rows are 1024 bytes apart. Begins on a 1024-byte boundary, or 32, 64, 96
 // bytes of k behind one.
 __device__ __forceinline__ uint64_t rows_k_major(unsigned address) { return (uint64_t)(address >> 4 & 0x3fff) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61; }
+// Columns of k of 16-bit elements, 64 side by side (128 bytes) a row of k in the copies' 128-byte swizzle: groups of 8 k are 1024 bytes apart, the next 64
+// elements `next` bytes. Begins on a 1024-byte boundary.
+__device__ __forceinline__ uint64_t columns_of_k(unsigned address, unsigned next) { return (uint64_t)(address >> 4 & 0x3fff) | (uint64_t)(next >> 4) << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61; }
+// D[128][N] (+)= A B^T over 16 k, 16-bit elements of one type (bf16 or fp16), both in columns of k
+__device__ __forceinline__ constexpr unsigned halves(unsigned n, bool bf16) { return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | 1u << 15 | 1u << 16 | (n >> 3) << 17 | (128u >> 4) << 24; }
+__device__ __forceinline__ void mma_halves(unsigned d, uint64_t a, uint64_t b, unsigned shape, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((unsigned)add)
+                 : "memory");
+}
 // 32 scales of 16 bytes, without swizzle: groups of 8 are 128 bytes apart
 __device__ __forceinline__ uint64_t scale_rows(unsigned address) { return (uint64_t)(address >> 4 & 0x3fff) | 8ull << 16 | 8ull << 32 | 1ull << 46; }
 // 512 bytes to 4 columns: lane l of each quarter gets bytes 16 l to 16 l + 15
