@@ -59,38 +59,27 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 16 elements that begin on a 16-byte boundary
-template <class T> __device__ __forceinline__ void load16(const T *p, float *v)
+// The 16 elements that lane `lane8` of 8 has of a row's block of 128 columns, and what becomes of them. vec: the row begins on a 16-byte
+// boundary and has the whole block; the lane then has pieces of 16 bytes, every eighth one, and otherwise every eighth element, so that the lanes read and
+// write side by side either way.
+template <class T> __device__ __forceinline__ unsigned column_in_block(int i, unsigned lane8, bool vec)
 {
     constexpr int per = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 16 / per; i++)
-    {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p + i * per);
-        const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-        for (int j = 0; j < per; j++) v[i * per + j] = to_float(e[j]);
-    }
+    return vec ? i / per * 8 * per + lane8 * per + i % per : 8 * i + lane8;
 }
-template <class T> __device__ __forceinline__ void store16(T *p, const float *v)
-{
-    constexpr int per = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 16 / per; i++)
-    {
-        uint4 w;
-        T *e = reinterpret_cast<T *>(&w);
-#pragma unroll
-        for (int j = 0; j < per; j++) e[j] = from_float<T>(v[i * per + j]);
-        *reinterpret_cast<uint4 *>(p + i * per) = w;
-    }
-}
-
-// The 16 elements that lane `lane8` of 8 has of a row's block of 128 columns. vec: the row begins on a 16-byte boundary and has the whole block; they are
-// columns 16 * lane8 + i, otherwise 8 * i + lane8, so that the eight lanes read side by side, with zeros behind the row's end.
+// (zeros behind the row's end)
 template <class T> __device__ __forceinline__ void load_block(const T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec, float *v)
 {
-    if (vec) load16(row + col0 + 16 * lane8, v);
+    constexpr int per = 16 / sizeof(T);
+    if (vec)
+    {
+        uint4 w[16 / per];
+#pragma unroll
+        for (int i = 0; i < 16 / per; i++) w[i] = *reinterpret_cast<const uint4 *>(row + col0 + column_in_block<T>(i * per, lane8, true));
+        const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = to_float(e[i]);
+    }
     else
 #pragma unroll
         for (int i = 0; i < 16; i++)
@@ -109,11 +98,19 @@ __device__ __forceinline__ float largest_of_8(const float *v)
     for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
     return most;
 }
-// what load_block gave, to 8 bits; `to` is the block's first byte, vec as in load_block (and the block inside the row)
-__device__ __forceinline__ void store_block(const float *v, bool vec, unsigned lane8, unsigned scale, uint8_t *to)
+// what load_block gave, to 8 bits; `to` is the block's first byte
+template <class T> __device__ __forceinline__ void store_block(const float *v, bool vec, unsigned lane8, unsigned scale, uint8_t *to)
 {
+    constexpr int per = 16 / sizeof(T);
     const float inv = inverse(scale);
-    if (vec) *reinterpret_cast<uint4 *>(to + 16 * lane8) = make_uint4(pack4(v, inv), pack4(v + 4, inv), pack4(v + 8, inv), pack4(v + 12, inv));
+    if (vec)
+#pragma unroll
+        for (int i = 0; i < 16; i += per)
+        {
+            uint8_t *at = to + column_in_block<T>(i, lane8, true);
+            if constexpr (per == 4) *reinterpret_cast<unsigned *>(at) = pack4(v + i, inv);
+            else *reinterpret_cast<uint2 *>(at) = make_uint2(pack4(v + i, inv), pack4(v + i + 4, inv));
+        }
     else
 #pragma unroll
         for (int i = 0; i < 16; i += 2)
@@ -121,6 +118,32 @@ __device__ __forceinline__ void store_block(const float *v, bool vec, unsigned l
             const unsigned two = pack2(v[i], v[i + 1], inv);
             to[8 * i + lane8] = (uint8_t)two;
             to[8 * (i + 1) + lane8] = (uint8_t)(two >> 8);
+        }
+}
+// the other way: a block in 8 bits to the caller's type
+template <class T> __device__ __forceinline__ void restore_block(const uint8_t *from, float scale, T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec)
+{
+    constexpr int per = 16 / sizeof(T);
+    if (vec)
+#pragma unroll
+        for (int i = 0; i < 16; i += per)
+        {
+            const unsigned c = column_in_block<T>(i, lane8, true);
+            float v[per];
+#pragma unroll
+            for (int k = 0; k < per; k += 4) unpack4(*reinterpret_cast<const unsigned *>(from + c + k), v + k);
+            uint4 w;
+            T *e = reinterpret_cast<T *>(&w);
+#pragma unroll
+            for (int k = 0; k < per; k++) e[k] = from_float<T>(v[k] * scale);
+            *reinterpret_cast<uint4 *>(row + col0 + c) = w;
+        }
+    else
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+        {
+            const unsigned c = 8 * i + lane8;
+            if (col0 + c < n_cols) row[col0 + c] = from_float<T>(__low2float(unpack2(from[c])) * scale);
         }
 }
 } // namespace block8

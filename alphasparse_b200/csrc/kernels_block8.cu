@@ -24,52 +24,35 @@ template <class T> bool vectors(const Dense &x) { return ((uintptr_t)x.p & 15) =
 
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
-// 32 rows x 512 columns to a CTA of 8 warps: a warp takes a row's four blocks at once, 8 lanes and 16 elements a lane each, so that an
-// element is read once and its block's largest is known after three exchanges. Bounded by memory. A row's four scales leave as a
-// word.
-constexpr int kQuantRows = 32;
+// A row's four blocks to a warp, 8 lanes and 16 elements a lane each, so that an element is read once, its block's largest is known after
+// three exchanges, and the four scales leave as a word. Bounded by memory. Eight rows to a CTA: no warp waits for another.
 template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const T *x, uint64_t ld, bool vec, unsigned n, Rows8Dev out)
 {
-    __shared__ __align__(4) uint8_t scales[kQuantRows][4];
-    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (out.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
-    const unsigned blk0 = blockIdx.x % fours * 4, blk = blk0 + lane / 8, row0 = blockIdx.x / fours * kQuantRows;
-#pragma unroll
-    for (int i = 0; i < kQuantRows / 8; i++)
-    {
-        const unsigned row = row0 + i * 8 + warp;
-        if (row >= n) break;
-        const bool there = blk < n_blocks, together = vec && (blk + 1) * 128 <= out.n_cols;
-        float v[16];
-        load_block(x + (uint64_t)row * ld, blk * 128, out.n_cols, lane8, together, v); // (zeros behind the last block)
-        const float most = largest_of_8(v);
-        if (!there) continue;
-        const unsigned scale = scale_of(most);
-        store_block(v, together, lane8, scale, out.values + (uint64_t)row * out.ld + blk * 128);
-        if (lane8 == 0) scales[i * 8 + warp][lane / 8] = (uint8_t)scale;
-    }
-    __syncthreads();
-    const unsigned r = threadIdx.x;
-    if (r < kQuantRows && row0 + r < n) // the four blocks' bytes are a word (those behind the last block are not used)
-        *reinterpret_cast<unsigned *>(out.scales + scale_at(out, row0 + r, blk0)) = *reinterpret_cast<const unsigned *>(scales[r]);
+    const unsigned lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (out.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
+    const unsigned blk0 = blockIdx.x % fours * 4, blk = blk0 + lane / 8, row = blockIdx.x / fours * 8 + threadIdx.x / 32;
+    grid_wait();
+    grid_release();
+    if (row >= n) return;
+    const bool together = vec && (blk + 1) * 128 <= out.n_cols;
+    float v[16];
+    load_block(x + (uint64_t)row * ld, blk * 128, out.n_cols, lane8, together, v); // (zeros behind the last block)
+    const unsigned scale = scale_of(largest_of_8(v));
+    if (blk < n_blocks) store_block<T>(v, together, lane8, scale, out.values + (uint64_t)row * out.ld + blk * 128);
+    unsigned four = scale << lane / 8 * 8;
+    four |= __shfl_xor_sync(~0u, four, 8);
+    four |= __shfl_xor_sync(~0u, four, 16);
+    if (lane == 0) *reinterpret_cast<unsigned *>(out.scales + scale_at(out, row, blk0)) = four; // (those behind the last block are not used)
 }
 
-// 16 columns to a thread, a block of 128 columns and 32 rows to a CTA
+// the same the other way
 template <class T> __global__ void __launch_bounds__(256) k_rows8_restore(Rows8Dev x, T *out, uint64_t ld, bool vec)
 {
-    const unsigned n_blocks = (x.n_cols + 127) / 128, blk = blockIdx.x % n_blocks, row = blockIdx.x / n_blocks * 32 + threadIdx.x / 8, col = blk * 128 + 16 * (threadIdx.x % 8);
-    if (row >= x.n || col >= x.n_cols) return;
-    const float scale = power(x.scales[scale_at(x, row, blk)]);
-    const uint4 q = *reinterpret_cast<const uint4 *>(x.values + (uint64_t)row * x.ld + col);
-    float v[16];
-    unpack4(q.x, v), unpack4(q.y, v + 4), unpack4(q.z, v + 8), unpack4(q.w, v + 12);
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] *= scale;
-    T *to = out + (uint64_t)row * ld + col;
-    if (vec && col + 16 <= x.n_cols) store16(to, v);
-    else
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (col + i < x.n_cols) to[i] = from_float<T>(v[i]);
+    const unsigned lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (x.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
+    const unsigned blk = blockIdx.x % fours * 4 + lane / 8, row = blockIdx.x / fours * 8 + threadIdx.x / 32;
+    grid_wait();
+    grid_release();
+    if (row >= x.n || blk >= n_blocks) return;
+    restore_block(x.values + (uint64_t)row * x.ld + blk * 128, power(x.scales[scale_at(x, row, blk)]), out + (uint64_t)row * ld, blk * 128, x.n_cols, lane8, vec && (blk + 1) * 128 <= x.n_cols);
 }
 
 // ---- the matrix's values --------------------------------------------------------------------------------------------
@@ -92,6 +75,8 @@ __global__ void __launch_bounds__(256) k_block8_set(const T *from, const unsigne
     const unsigned rows = min(128u, n_rows - row[b] * 128), cols = min(128u, n_cols - col[b] * 128); // inside the matrix
     float v[8][8];
     float most = 0.f;
+    grid_wait();
+    grid_release();
 #pragma unroll
     for (int i = 0; i < 8; i++)
     {
@@ -143,17 +128,23 @@ __global__ void __launch_bounds__(256) k_block8_set(const T *from, const unsigne
     }
 }
 
-__global__ void __launch_bounds__(256) k_block8_get(const uint8_t *values, const uint8_t *scales, float *out, unsigned n_blocks)
+// four elements and 16 bytes a thread, four times
+__global__ void __launch_bounds__(256) k_block8_get(const uint8_t *values, const uint8_t *scales, float *out)
 {
-    // 16 elements a thread
-    const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 16;
-    const float scale = power(scales[at / 16384]);
-    const uint4 q = *reinterpret_cast<const uint4 *>(values + at);
-    float v[16];
-    unpack4(q.x, v), unpack4(q.y, v + 4), unpack4(q.z, v + 8), unpack4(q.w, v + 12);
+    const uint64_t at = (uint64_t)blockIdx.x * 4096 + threadIdx.x * 4;
+    grid_wait();
+    grid_release();
+    const float scale = power(scales[blockIdx.x / 4]);
+    unsigned q[4];
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] *= scale;
-    store16(out + at, v);
+    for (int i = 0; i < 4; i++) q[i] = *reinterpret_cast<const unsigned *>(values + at + i * 1024);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        float v[4];
+        unpack4(q[i], v);
+        *reinterpret_cast<float4 *>(out + at + i * 1024) = make_float4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
+    }
 }
 
 // ---- products with a few rows ----------------------------------------------------------------------------------------
@@ -204,7 +195,7 @@ struct Held // X is in 8 bits already
 {
 };
 
-template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_block8_few(const FewArgs args)
+template <int NT, class X, class Y> __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_block8_few(const FewArgs args)
 {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) unsigned char raw[];
@@ -247,11 +238,16 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
                 acc[nt][2 + i] = __fmaf_rn(c[nt][2 + i] * f1, f2, acc[nt][2 + i]);
             }
     };
+    // Until the kernels before this one are done the matrix may still be written: it is brought to L2, which is never behind, and read afterwards.
+    if (threadIdx.x == 0 && j0 < j1 && blockIdx.y == 0)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(args.a.values + (uint64_t)j0 * 16384), "r"(min(j1 - j0, 8u) * 16384) : "memory");
+    for (unsigned i = threadIdx.x; i < sizeof(sh.x) / 16; i += 256) reinterpret_cast<uint4 *>(sh.x)[i] = make_uint4(0, 0, 0, 0);
+    for (unsigned i = threadIdx.x; i < sizeof(sh.scale); i += 256) (&sh.scale[0][0])[i] = 127;
+    grid_wait();
+    grid_release();
     uint4 w0[4], w1[4];
     load(w0, j0);
     load(w1, j0 + 1);
-    for (unsigned i = threadIdx.x; i < sizeof(sh.x) / 16; i += 256) reinterpret_cast<uint4 *>(sh.x)[i] = make_uint4(0, 0, 0, 0);
-    for (unsigned i = threadIdx.x; i < sizeof(sh.scale); i += 256) (&sh.scale[0][0])[i] = 127;
     for (unsigned j = j0; j < j1; j += 2)
     {
         if ((j - j0) % kFewChunk == 0)
@@ -275,7 +271,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
                     const bool vec = args.vec && (kb + 1) * 128 <= args.a.n_cols;
                     load_block(reinterpret_cast<const X *>(args.x) + (uint64_t)(t0 + t) * args.ldx, kb * 128, args.a.n_cols, lane8, vec, v);
                     const unsigned scale = scale_of(largest_of_8(v));
-                    store_block(v, vec, lane8, scale, to);
+                    store_block<X>(v, vec, lane8, scale, to);
                     if (lane8 == 0) sh.scale[slot][t] = (uint8_t)scale;
                 }
             }
@@ -317,12 +313,14 @@ template <int NT, class X, class Y> cudaError_t few(const FewArgs &args, cudaStr
     cfg.blockDim = 256;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = args.n_split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, args);
 }
 template <class X, class Y> cudaError_t few_by_rows(const FewArgs &args, cudaStream_t st)
@@ -338,9 +336,8 @@ cudaError_t launch_rows8_quantize(const Dense &x, unsigned n, const Rows8Dev &ou
     if (n == 0) return cudaSuccess;
     return by_type(x.dtype, [&](auto t) {
         using T = decltype(t);
-        const unsigned grid = (out.n_cols + 511) / 512 * ((n + kQuantRows - 1) / kQuantRows);
-        k_rows8_quantize<T><<<grid, 256, 0, st>>>(reinterpret_cast<const T *>(x.p), x.ld, vectors<T>(x), n, out);
-        return cudaGetLastError();
+        const unsigned grid = (out.n_cols + 511) / 512 * ((n + 7) / 8);
+        return launch_pdl(k_rows8_quantize<T>, dim3(grid), dim3(256), 0, st, (const T *)x.p, x.ld, vectors<T>(x), n, out);
     });
 }
 
@@ -349,8 +346,8 @@ cudaError_t launch_rows8_restore(const Rows8Dev &x, const Dense &out, cudaStream
     if (x.n == 0) return cudaSuccess;
     return by_type(out.dtype, [&](auto t) {
         using T = decltype(t);
-        k_rows8_restore<T><<<(x.n_cols + 127) / 128 * ((x.n + 31) / 32), 256, 0, st>>>(x, reinterpret_cast<T *>(out.p), out.ld, vectors<T>(out));
-        return cudaGetLastError();
+        const unsigned grid = (x.n_cols + 511) / 512 * ((x.n + 7) / 8);
+        return launch_pdl(k_rows8_restore<T>, dim3(grid), dim3(256), 0, st, x, (T *)out.p, out.ld, vectors<T>(out));
     });
 }
 
@@ -359,16 +356,14 @@ cudaError_t launch_block8_set(const Block8Dev &a, const unsigned *row, const uns
     if (first >= end) return cudaSuccess;
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        k_block8_set<T><<<end - first, 256, 0, st>>>(reinterpret_cast<const T *>(from), row, a.col, place, to[0], to[1], first, a.n_rows, a.n_cols);
-        return cudaGetLastError();
+        return launch_pdl(k_block8_set<T>, dim3(end - first), dim3(256), 0, st, (const T *)from, row, a.col, place, to[0], to[1], first, a.n_rows, a.n_cols);
     });
 }
 
 cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st)
 {
     if (a.n_blocks == 0) return cudaSuccess;
-    k_block8_get<<<a.n_blocks * 4, 256, 0, st>>>(a.values, a.scales, out, a.n_blocks);
-    return cudaGetLastError();
+    return launch_pdl(k_block8_get, dim3(a.n_blocks * 4), dim3(256), 0, st, a.values, a.scales, out);
 }
 
 cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, cudaStream_t st)

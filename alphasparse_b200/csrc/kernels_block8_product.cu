@@ -6,6 +6,7 @@
 #include "../../include/asp_b200.h"
 #include "block8.h"
 #include "block8_device.h"
+#include "launch.h"
 #include "tcgen05.h"
 #include "tensor_map.h"
 
@@ -117,7 +118,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
     extern __shared__ unsigned char raw[];
     __shared__ Shared sh;
     unsigned char *stages = raw + (1024 - tc::shared_address(raw) % 1024) % 1024;
-    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const unsigned warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    if (threadIdx.x == 32) tc::prefetch_map(&map_a), tc::prefetch_map(&map_x);
     if (threadIdx.x == 0)
     {
         for (unsigned i = 0; i < p.stages; i++)
@@ -138,13 +140,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
     __syncthreads();
     tc::fence_after();
     const unsigned tensor = sh.tensor;
+    grid_wait();
+    grid_release();
     const unsigned x_bytes = p.tile * 128;
 
     if (warp == 0)
     {
-        if (lane == 0)
+        if (tc::one_lane())
         {
-            tc::prefetch_map(&map_a), tc::prefetch_map(&map_x);
             unsigned s = 0, phase = 0;
             for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
                 for (; at.j < at.end; at.j++)
@@ -165,35 +168,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
     }
     else if (warp == 1)
     {
-        if (lane == 0)
+        if (tc::one_lane())
         {
+            // A step's copies are waited for under the products of the step before: a look at a barrier takes a hundred clocks and more, and the tensor cores
+            // have no more than two or three products waiting.
             unsigned s = 0, phase = 0, b = 0, b_phase = 0, turn = 0;
+            bool ready = false;
             for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
             {
                 if (at.j == at.end) continue;
                 if (!tc::barrier_wait(&sh.taken[b], b_phase ^ 1, &sh.gave_up)) goto end;
-                tc::fence_after();
                 const unsigned d = tensor + b * kMostRows, shift = at.t0 % 128 / 32; // (of the first row among its piece's columns)
                 bool add = false;
                 for (; at.j < at.end; at.j++)
                 {
                     const unsigned shape = tc::scaled_e4m3(p.tile, p.a.col[at.j] % 4);
-                    if (!tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
+                    if (!ready && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
                     tc::fence_after();
                     const unsigned a = tc::shared_address(stages + s * p.stage_bytes), x = a + 16384, scales = x + x_bytes;
                     const unsigned sa = tensor + 2 * kMostRows + turn * 4, sx = tensor + 2 * kMostRows + 8 + turn * 8;
+                    uint64_t *const empty = &sh.empty[s];
+                    if (++s == p.stages) s = 0, phase ^= 1;
                     tc::copy_scales(sa, tc::scale_rows(scales));
                     tc::copy_scales(sx, tc::scale_rows(scales + 512));
                     if (shift + p.tile / 32 > 4) tc::copy_scales(sx + 4, tc::scale_rows(scales + 1024));
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                     {
+                        if (k == 1)
+                        {
+                            ready = at.j + 1 < at.end;
+                            if (ready && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
+                        }
                         tc::mma_scaled(d, tc::rows_k_major(a + 32 * k), tc::rows_k_major(x + 32 * k), shape, sa, sx + shift, add);
                         add = true;
                     }
-                    tc::commit(&sh.empty[s]);
+                    tc::commit(empty);
                     turn ^= 1;
-                    if (++s == p.stages) s = 0, phase ^= 1;
                 }
                 tc::commit(&sh.done[b]);
                 b ^= 1;
@@ -216,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
                 for (unsigned c = first; c < p.tile; c += 64) store_columns<Y>(v, p, row0, lane, at.t0 + c, limit);
                 continue;
             }
-            if (!tc::barrier_wait(&sh.done[b], b_phase, &sh.gave_up)) break;
+            if (!tc::barrier_wait<64>(&sh.done[b], b_phase, &sh.gave_up)) break;
             tc::fence_after();
             for (unsigned c = first; c < p.tile; c += 64)
             {
@@ -266,8 +277,7 @@ template <class Y> cudaError_t product(const CUtensorMap &map_a, const CUtensorM
     const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
     const cudaError_t e = cudaFuncSetAttribute(k_block8_product<Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    k_block8_product<Y><<<std::min<unsigned>(p.n_tiles, (unsigned)sm_count), kThreads, smem, st>>>(map_a, map_x, p);
-    return cudaGetLastError();
+    return launch_pdl(k_block8_product<Y>, dim3(std::min<unsigned>(p.n_tiles, (unsigned)sm_count)), dim3(kThreads), smem, st, map_a, map_x, p);
 }
 } // namespace
 

@@ -13,6 +13,15 @@ namespace tc
 {
 __device__ __forceinline__ unsigned shared_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 
+// One lane of the warp, which is here as a whole. The compiler knows that what follows runs in one lane and issues copies and products as they
+// are; behind a test of the lane's number it goes through the lanes for each of them (measured: 490 clocks for what takes 50).
+__device__ __forceinline__ bool one_lane()
+{
+    unsigned one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // ---- barriers ----
 __device__ __forceinline__ void barrier_init(uint64_t *b, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory"); }
 __device__ __forceinline__ void barrier_arrive(uint64_t *b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(b)) : "memory"); }
@@ -34,12 +43,14 @@ __device__ __forceinline__ uint64_t now_ns()
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-__device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile unsigned *gave_up)
+// idle_ns: what a warp that waits for long sleeps between two looks, so that it does not take issue slots from those that work
+template <unsigned idle_ns = 0> __device__ __forceinline__ bool barrier_wait(uint64_t *b, unsigned parity, volatile unsigned *gave_up)
 {
     if (barrier_test(b, parity)) return true;
     uint64_t since = 0;
     for (unsigned i = 1;; i++)
     {
+        if (idle_ns) __nanosleep(idle_ns);
         if (barrier_test(b, parity)) return true;
         if (i % 256) continue;
         if (*gave_up) return false;
