@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+#include <string.h>
 
 namespace asp
 {
@@ -27,16 +28,17 @@ __device__ __forceinline__ unsigned scale_of(float most)
 __device__ __forceinline__ float power(unsigned scale) { return __uint_as_float(scale << 23); }            // 2^k
 __device__ __forceinline__ float inverse(unsigned scale) { return __uint_as_float((254u - scale) << 23); } // 2^-k; scale is 1 to 247
 
-// Two elements to e4m3, `a` in the low byte. The conversion saturates: what is infinite is made NaN first (v - v is NaN then, else 0).
-__device__ __forceinline__ unsigned pack2(float a, float b, float inv)
+// Two elements to e4m3, `a` in the low byte; NaN stays NaN. The conversion saturates: where an element may be infinite it is made NaN first
+// (v - v is NaN then, else 0).
+template <bool infinite> __device__ __forceinline__ unsigned pack2(float a, float b, float inv)
 {
     unsigned short r;
-    a = __fmaf_rn(a, inv, a - a);
-    b = __fmaf_rn(b, inv, b - b);
+    a = infinite ? __fmaf_rn(a, inv, a - a) : a * inv;
+    b = infinite ? __fmaf_rn(b, inv, b - b) : b * inv;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
     return r;
 }
-__device__ __forceinline__ unsigned pack4(const float *v, float inv) { return pack2(v[0], v[1], inv) | pack2(v[2], v[3], inv) << 16; }
+template <bool infinite> __device__ __forceinline__ unsigned pack4(const float *v, float inv) { return pack2<infinite>(v[0], v[1], inv) | pack2<infinite>(v[2], v[3], inv) << 16; }
 
 // two e4m3 (exact in fp16, NaN included)
 __device__ __forceinline__ __half2 unpack2(unsigned two)
@@ -67,58 +69,78 @@ template <class T> __device__ __forceinline__ unsigned column_in_block(int i, un
     constexpr int per = 16 / sizeof(T);
     return vec ? i / per * 8 * per + lane8 * per + i % per : 8 * i + lane8;
 }
-// (zeros behind the row's end)
-template <class T> __device__ __forceinline__ void load_block(const T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec, float *v)
+// as they lie in memory, zeros behind the row's end
+template <class T> struct Raw
 {
-    constexpr int per = 16 / sizeof(T);
-    if (vec)
+    uint4 w[sizeof(T)];
+    __device__ __forceinline__ void load(const T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec)
     {
-        uint4 w[16 / per];
+        constexpr int per = 16 / sizeof(T);
+        if (vec)
 #pragma unroll
-        for (int i = 0; i < 16 / per; i++) w[i] = *reinterpret_cast<const uint4 *>(row + col0 + column_in_block<T>(i * per, lane8, true));
-        const T *e = reinterpret_cast<const T *>(w);
+            for (int i = 0; i < 16 / per; i++) w[i] = *reinterpret_cast<const uint4 *>(row + col0 + column_in_block<T>(i * per, lane8, true));
+        else
+        {
+            T e[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+            {
+                const unsigned c = col0 + 8 * i + lane8;
+                e[i] = c < n_cols ? row[c] : from_float<T>(0.f);
+            }
+            memcpy(w, e, sizeof(w));
+        }
+    }
+    __device__ __forceinline__ void floats(float *v) const
+    {
+        T e[16];
+        memcpy(e, w, sizeof(w));
 #pragma unroll
         for (int i = 0; i < 16; i++) v[i] = to_float(e[i]);
     }
-    else
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-        {
-            const unsigned c = col0 + 8 * i + lane8;
-            v[i] = c < n_cols ? to_float(row[c]) : 0.f;
-        }
-}
-// the largest finite magnitude of what the eight lanes of a block have; all lanes of the warp take part
-__device__ __forceinline__ float largest_of_8(const float *v)
+};
+// The scale of what the eight lanes of a block have, and whether something infinite is among it. All lanes of the warp take part. (fmaxf passes NaN over;
+// only what is infinite takes a second look.)
+__device__ __forceinline__ unsigned scale_of_8(const float *v, bool &infinite)
 {
     float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) most = fmaxf(most, finite_size(v[i]));
+    for (int i = 0; i < 16; i++) most = fmaxf(most, fabsf(v[i]));
 #pragma unroll
     for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-    return most;
+    infinite = __any_sync(~0u, isinf(most));
+    if (infinite)
+    {
+        most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) most = fmaxf(most, finite_size(v[i]));
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    }
+    return scale_of(most);
 }
-// what load_block gave, to 8 bits; `to` is the block's first byte
-template <class T> __device__ __forceinline__ void store_block(const float *v, bool vec, unsigned lane8, unsigned scale, uint8_t *to)
+// to 8 bits, four to a word, in the order of `v`
+__device__ __forceinline__ void pack16(const float *v, unsigned scale, bool infinite, unsigned *q)
+{
+    const float inv = inverse(scale);
+#pragma unroll
+    for (int i = 0; i < 4; i++) q[i] = infinite ? pack4<true>(v + 4 * i, inv) : pack4<false>(v + 4 * i, inv);
+}
+// and to where they belong; `to` is the block's first byte
+template <class T> __device__ __forceinline__ void store_block(const unsigned *q, bool vec, unsigned lane8, uint8_t *to)
 {
     constexpr int per = 16 / sizeof(T);
-    const float inv = inverse(scale);
     if (vec)
 #pragma unroll
         for (int i = 0; i < 16; i += per)
         {
             uint8_t *at = to + column_in_block<T>(i, lane8, true);
-            if constexpr (per == 4) *reinterpret_cast<unsigned *>(at) = pack4(v + i, inv);
-            else *reinterpret_cast<uint2 *>(at) = make_uint2(pack4(v + i, inv), pack4(v + i + 4, inv));
+            if constexpr (per == 4) *reinterpret_cast<unsigned *>(at) = q[i / 4];
+            else *reinterpret_cast<uint2 *>(at) = make_uint2(q[i / 4], q[i / 4 + 1]);
         }
     else
 #pragma unroll
-        for (int i = 0; i < 16; i += 2)
-        {
-            const unsigned two = pack2(v[i], v[i + 1], inv);
-            to[8 * i + lane8] = (uint8_t)two;
-            to[8 * (i + 1) + lane8] = (uint8_t)(two >> 8);
-        }
+        for (int i = 0; i < 16; i++) to[8 * i + lane8] = (uint8_t)(q[i / 4] >> 8 * (i % 4));
 }
 // the other way: a block in 8 bits to the caller's type
 template <class T> __device__ __forceinline__ void restore_block(const uint8_t *from, float scale, T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec)

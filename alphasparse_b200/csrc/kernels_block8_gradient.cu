@@ -330,7 +330,8 @@ end:
 template <class Unfold> cudaError_t gradient(const CUtensorMap &map_dy, const CUtensorMap &map_x, const GradientArgs &p, int sm_count, cudaStream_t st)
 {
     const size_t smem = kStages * kStageBytes + kUnfolded * kUnfoldedBytes + kHeld * kHeldBytes + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(k_block8_gradient<Unfold>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SharedAllowance allowance;
+    const cudaError_t e = allowance.need((const void *)k_block8_gradient<Unfold>, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_block8_gradient<Unfold>, dim3(std::min<unsigned>(p.n_pairs, (unsigned)sm_count)), dim3(kThreads), smem, st, map_dy, map_x, p);
 }

@@ -275,7 +275,8 @@ unsigned tile_rows(const Block8Dev &a, unsigned n, int sm_count)
 template <class Y> cudaError_t product(const CUtensorMap &map_a, const CUtensorMap &map_x, const ProductArgs &p, int sm_count, cudaStream_t st)
 {
     const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(k_block8_product<Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SharedAllowance allowance;
+    const cudaError_t e = allowance.need((const void *)k_block8_product<Y>, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_block8_product<Y>, dim3(std::min<unsigned>(p.n_tiles, (unsigned)sm_count)), dim3(kThreads), smem, st, map_a, map_x, p);
 }

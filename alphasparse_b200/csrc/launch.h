@@ -17,6 +17,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 namespace asp
 {
 #ifdef __CUDACC__
@@ -49,6 +51,24 @@ __device__ __forceinline__ double ld_x(const double *p)
     asm volatile("ld.global.f64 %0, [%1];" : "=d"(v) : "l"(p));
     return v;
 }
+
+// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) of one kernel, once per device and size instead of with every launch (0.3 us)
+class SharedAllowance
+{
+    std::atomic<int> given[64] = {};
+
+  public:
+    cudaError_t need(const void *kernel, int bytes)
+    {
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e != cudaSuccess) return e;
+        if (device < 64 && given[device].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && device < 64) given[device].store(bytes, std::memory_order_relaxed);
+        return e;
+    }
+};
 
 template <class... A>
 cudaError_t launch_pdl(void (*kernel)(A...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
