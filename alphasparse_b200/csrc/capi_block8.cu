@@ -38,7 +38,8 @@ struct asp_block8
     Room room;
     asp::host::Block8Pattern pattern;
     asp::Block8Dev side[2] = {};
-    const unsigned *row = nullptr, *place = nullptr, *pairs = nullptr;
+    const unsigned *row = nullptr, *place = nullptr;
+    asp::Block8Groups groups = {};
     asp::Block8Set set[2] = {};
     bool transposed = false;
     size_t bytes = 0;
@@ -104,7 +105,9 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
         col[s] = take(n * 4);
         order[s] = take(p.side[s].order.size() * 4);
     }
-    const Piece row = take(n * 4), place = take(n * 4), pairs = take(p.pairs.size() * 4);
+    const Piece row = take(n * 4), place = take(n * 4), from = take(n * 4);
+    Piece groups[4];
+    for (int g = 0; g < 4; g++) groups[g] = take(p.groups[g].size() * 4);
     std::vector<uint32_t> rows(n);
     for (uint32_t r = 0; r < p.side[0].rows(); r++) std::fill(rows.begin() + p.side[0].ptr[r], rows.begin() + p.side[0].ptr[r + 1], r);
     ASP_ON_DEVICE(ctx);
@@ -141,7 +144,14 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
     }
     m->row = send(row, rows.data());
     m->place = send(place, p.place.data());
-    m->pairs = send(pairs, p.pairs.data());
+    m->groups.row = m->row, m->groups.col = m->side[0].col;
+    m->groups.from = send(from, p.from.data());
+    for (int g = 0; g < 4; g++)
+    {
+        m->groups.groups[g] = send(groups[g], p.groups[g].data());
+        m->groups.count[g] = (unsigned)p.groups[g].size();
+        std::copy(p.sizes[g], p.sizes[g] + 4, m->groups.sizes[g]);
+    }
     e = ctx->stager.to_device(m->room.base, segments, ctx->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) return cuda_fail(e, "upload of the pattern");
@@ -365,7 +375,7 @@ asp_status asp_block8_gradient(asp_ctx *ctx, const asp_block8 *m, const asp_rows
     ASP_TRY(same_device(ctx, m->room));
     ASP_TRY(same_device(ctx, x->room));
     ASP_ON_DEVICE(ctx);
-    return launched(asp::launch_block8_gradient(m->side[0], m->row, m->pairs, (unsigned)m->pattern.pairs.size(), x->dev, dy, d_out, accumulate != 0, ctx->sm_count, ctx->fault, ctx->stream));
+    return launched(asp::launch_block8_gradient(m->side[0], m->groups, x->dev, dy, d_out, accumulate != 0, ctx->sm_count, ctx->fault, ctx->stream));
 }
 
 } // extern "C"

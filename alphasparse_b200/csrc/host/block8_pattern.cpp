@@ -64,8 +64,23 @@ asp_status make_pattern(u64 n_rows, u64 n_cols, const int64_t *block_ptr, const 
             out.place[j] = next[a.col[j]]++;
             t.col[out.place[j]] = r;
         }
-    for (u64 r = 0; r < nr; r++)
-        for (u32 j = a.ptr[r]; j < a.ptr[r + 1]; j += 2) out.pairs.push_back(j | (j + 1 < a.ptr[r + 1] ? 1u << 31 : 0u));
+    out.from.resize(n);
+    for (u64 j = 0; j < n; j++) out.from[out.place[j]] = (u32)j;
+    for (u32 most = 1; most <= 4; most++)
+    {
+        std::vector<u32> &g = out.groups[most - 1];
+        for (u64 c = 0; c < nc; c++)
+        {
+            const u32 lo = t.ptr[c], len = t.ptr[c + 1] - lo, parts = (len + most - 1) / most;
+            for (u32 k = 0; k < parts; k++)
+            {
+                const u32 begin = (u32)((u64)len * k / parts), size = (u32)((u64)len * (k + 1) / parts) - begin;
+                g.push_back((lo + begin) | (size - 1) << 24);
+                out.sizes[most - 1][size - 1]++;
+            }
+        }
+        std::stable_sort(g.begin(), g.end(), [](u32 x, u32 y) { return x >> 24 > y >> 24; });
+    }
     finish(a);
     finish(t);
     return ASP_OK;

@@ -394,20 +394,7 @@ template <int NT, class X, class Y> cudaError_t few(const FewArgs &args, cudaStr
     static SharedAllowance allowance;
     const cudaError_t e = allowance.need((const void *)kernel, (int)smem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(args.a.n_block_rows * args.n_split, (args.n + 8 * NT - 1) / (8 * NT));
-    cfg.blockDim = 256;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = args.n_split;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, args);
+    return launch_pdl_cluster(kernel, args.n_split, dim3(args.a.n_block_rows * args.n_split, (args.n + 8 * NT - 1) / (8 * NT)), dim3(256), smem, st, args);
 }
 template <class X, class Y> cudaError_t few_by_rows(const FewArgs &args, cudaStream_t st)
 {

@@ -71,20 +71,28 @@ class SharedAllowance
 };
 
 template <class... A>
-cudaError_t launch_pdl(void (*kernel)(A...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
+cudaError_t launch_pdl_cluster(void (*kernel)(A...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     void *p[] = {(void *)&args...};
     return cudaLaunchKernelExC(&cfg, (const void *)kernel, p);
+}
+template <class... A>
+cudaError_t launch_pdl(void (*kernel)(A...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
+{
+    return launch_pdl_cluster(kernel, 1, grid, block, smem, st, args...);
 }
 #endif
 } // namespace asp
