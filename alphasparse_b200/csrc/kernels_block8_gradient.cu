@@ -31,7 +31,10 @@ using namespace block8;
 constexpr unsigned kRows = 64;          // t a step
 constexpr unsigned kTile = kRows * 128; // bytes of 64 columns of a step's rows in 16 bits, of 128 in 8
 constexpr unsigned kRoom = 8, kBlockBytes = 2 * kTile;        // dy: blocks of a step's rows, as many steps as fit
-constexpr unsigned kHeld = 3, kHeldBytes = kTile + 1024;      // x in 8 bits, and its scales
+constexpr unsigned kHeld = 4, kHeldBytes = kTile + 1024;      // x in 8 bits, and its scales
+// A place for x belongs to one of the two groups that unfold it. Were it to change hands, the group that is two steps ahead might look for the second of two
+// copies to a place before the first has arrived (they may overtake one another), and take the one before both, of the same parity, for it.
+static_assert(kHeld % 2 == 0, "places for x are shared out between two groups of warps");
 constexpr unsigned kUnfolded = 3, kUnfoldedBytes = 2 * kTile; // x in 16 bits: 64 columns after 64 columns, a row t 128 bytes
 constexpr unsigned kThreads = 640;
 
