@@ -289,16 +289,24 @@ end:
             const bool inside = col * 128 + c < p.n_cols;
             for (unsigned d = part * width + (warp - 4) / 4 * 32; d < (part + 1) * width; d += 128)
             {
-                float v[32];
-                tc::tensor_load32(tensor + d + (quarter * 32 << 16), v);
+                float v[32], o[32];
                 const unsigned b = p.groups.from[first + d / 128], r0 = d % 128, rows = p.n_rows - p.groups.row[b] * 128;
                 float *to = p.out + (uint64_t)b * 16384 + r0 * 128 + c;
-                const bool add = p.accumulate || turn > 0;
-#pragma unroll
-                for (unsigned k = 0; k < 32; k++)
+                if (p.accumulate || turn > 0) // (all of them on their way before the first is needed)
                 {
-                    const float o = add ? __ldcg(to + k * 128) : 0.f;
-                    __stcg(to + k * 128, (inside && r0 + k < rows ? v[k] : 0.f) + o); // zero outside the matrix
+#pragma unroll
+                    for (unsigned k = 0; k < 32; k++) o[k] = __ldcg(to + k * 128);
+                }
+                tc::tensor_load32(tensor + d + (quarter * 32 << 16), v);
+                if (p.accumulate || turn > 0)
+                {
+#pragma unroll
+                    for (unsigned k = 0; k < 32; k++) __stcg(to + k * 128, (inside && r0 + k < rows ? v[k] : 0.f) + o[k]); // zero outside the matrix
+                }
+                else
+                {
+#pragma unroll
+                    for (unsigned k = 0; k < 32; k++) __stcg(to + k * 128, inside && r0 + k < rows ? v[k] : 0.f);
                 }
             }
         }
