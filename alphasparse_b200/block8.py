@@ -43,6 +43,17 @@ def _lib():
     return _bound
 
 
+def _bind_apply(ctx_handle, handle):
+    """asp_block8_apply(ctx, matrix, ...) with the first two given, without ctypes where that binding has been built. Both handles are read at every
+    call; the caller keeps them alive."""
+    try:
+        native = capi._native().Apply
+    except (ImportError, AttributeError):
+        fn = _lib().asp_block8_apply
+        return lambda *args: fn(ctx_handle, handle, *args)
+    return native(C.cast(_lib().asp_block8_apply, C.c_void_p).value, C.addressof(ctx_handle), C.addressof(handle))
+
+
 class Rows8:
     """asp_rows8: up to max_rows rows of n_cols columns in 8 bits, a scale for each row and 128 columns."""
 
@@ -99,6 +110,8 @@ class Block8:
 
     def _take(self, ctx, h, n_rows, n_cols):
         self._h, self.ctx, self.n_rows, self.n_cols = h, ctx, n_rows, n_cols
+        self._ctx_handle = ctx.handle  # kept alive: _call may have no more than its address and that of our own
+        self._apply = _bind_apply(self._ctx_handle, h)
         self.n_blocks = int(_lib().asp_block8_blocks(h))
 
     def pattern(self):
@@ -120,7 +133,13 @@ class Block8:
 
     def apply(self, x: int, n: int, x_dtype: str, y: int, y_dtype: str, ldx: int = 0, ldy: int = 0, transposed: bool = False) -> None:
         """y = A x (transposed: A^T x) for n <= 32 rows x in 16 or 32 bits, converted to 8 bits on the way."""
-        capi.check(_lib().asp_block8_apply(self.ctx.handle, self._h, transposed, x, TYPES[x_dtype], n, ldx, y, TYPES[y_dtype], ldy))
+        args = (transposed, x, TYPES[x_dtype], n, ldx, y, TYPES[y_dtype], ldy)
+        try:
+            status = self._apply(*args)
+        except TypeError:  # whatever else ctypes takes for a pointer
+            status = _lib().asp_block8_apply(self.ctx.handle, self._h, *args)
+        if status:
+            capi.check(status)
 
     def product(self, x: Rows8, y: int, dtype: str, ld: int = 0, transposed: bool = False) -> None:
         """y = A x (transposed: A^T x) for the rows that x holds."""
@@ -133,7 +152,7 @@ class Block8:
     def close(self):
         if self._h:
             _lib().asp_block8_destroy(self._h)
-            self._h = C.c_void_p()
+            self._h.value = None  # (in place: its address is held)
 
     def __del__(self):
         try:

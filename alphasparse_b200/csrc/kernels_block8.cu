@@ -380,8 +380,11 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     for (unsigned i = threadIdx.x + 256 * piece; i < tokens * 128; i += 256 * split)
     {
         const unsigned t = i / 128, r = i % 128;
-        float sum = 0.f;
-        for (unsigned s = 0; s < split; s++) sum += *cluster.map_shared_rank(&sh.part[t][r], s);
+        float v[8], sum = 0.f; // all on their way before the first is needed
+#pragma unroll
+        for (unsigned s = 0; s < 8; s++) v[s] = s < split ? *cluster.map_shared_rank(&sh.part[t][r], s) : 0.f;
+#pragma unroll
+        for (unsigned s = 0; s < 8; s++) sum += v[s]; // (in order; zeros behind the last change nothing)
         if (br * 128 + r < args.a.n_rows) y[(uint64_t)(t0 + t) * args.ldy + br * 128 + r] = from_float<Y>(sum);
     }
     cluster.sync(); // (its shared memory is read until here)

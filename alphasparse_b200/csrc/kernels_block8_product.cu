@@ -10,6 +10,8 @@
 #include "tcgen05.h"
 #include "tensor_map.h"
 
+#include <cooperative_groups.h>
+
 namespace asp
 {
 namespace
@@ -24,6 +26,9 @@ using namespace block8;
 // rows of D because a block is 128 rows of A whatever the pattern, while X can be cut anywhere; 192 since two tiles' sums (384
 // columns) and the scales (24) then share the 512 columns, so that a tile is stored under the next one's products, and whole 64s since the
 // scales of X begin at every second column.
+//
+// Where there are fewer tiles than SMs, a cluster shares the blocks of a tile; its CTAs put their sums into shared memory and add them up in order,
+// some columns each.
 //
 // A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 9 store.
 constexpr unsigned kMostRows = 192;
@@ -41,6 +46,7 @@ struct ProductArgs
     unsigned tile;   // rows of X a tile, a multiple of 64
     unsigned tiles_x, group;
     unsigned n_tiles;
+    unsigned split;  // CTAs that share a tile's blocks; then a CTA has one tile
     unsigned stages, stage_bytes;
     bool pairs;      // two 16-bit elements of y at a time
     unsigned *fault;
@@ -58,7 +64,7 @@ struct Steps
 {
     const ProductArgs &p;
     unsigned tile, j = 0, end = 0, row = 0, t0 = 0;
-    __device__ __forceinline__ Steps(const ProductArgs &args, unsigned first) : p(args), tile(first) { locate(); }
+    __device__ __forceinline__ explicit Steps(const ProductArgs &args) : p(args), tile(blockIdx.x / args.split) { locate(); }
     __device__ __forceinline__ bool valid() const { return tile < p.n_tiles; }
     __device__ __forceinline__ void locate()
     {
@@ -66,11 +72,12 @@ struct Steps
         const unsigned per = p.group * p.tiles_x, g = tile / per, in = tile % per, rows = min(p.group, p.a.n_block_rows - g * p.group);
         row = p.a.order[g * p.group + in % rows];
         t0 = in / rows * p.tile;
-        j = p.a.ptr[row], end = p.a.ptr[row + 1];
+        const unsigned lo = p.a.ptr[row], len = p.a.ptr[row + 1] - lo, piece = blockIdx.x % p.split;
+        j = lo + len * piece / p.split, end = lo + len * (piece + 1) / p.split; // (less than 2^24 blocks, 8 pieces at most)
     }
     __device__ __forceinline__ void next_tile()
     {
-        tile += gridDim.x;
+        tile += gridDim.x / p.split;
         locate();
     }
 };
@@ -149,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
         if (tc::one_lane())
         {
             unsigned s = 0, phase = 0;
-            for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
+            for (Steps at(p); at.valid(); at.next_tile())
                 for (; at.j < at.end; at.j++)
                 {
                     const unsigned col = p.a.col[at.j];
@@ -174,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
             // have no more than two or three products waiting.
             unsigned s = 0, phase = 0, b = 0, b_phase = 0, turn = 0;
             bool ready = false;
-            for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
+            for (Steps at(p); at.valid(); at.next_tile())
             {
                 if (at.j == at.end) continue;
                 if (!tc::barrier_wait(&sh.taken[b], b_phase ^ 1, &sh.gave_up)) goto end;
@@ -216,10 +223,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
     {
         unsigned b = 0, b_phase = 0;
         const unsigned quarter = warp % 4, first = (warp - 2) / 4 * 32; // two warps to a quarter of D's lanes, every second 32 columns each
-        for (Steps at(p, blockIdx.x); at.valid(); at.next_tile())
+        for (Steps at(p); at.valid(); at.next_tile())
         {
             const unsigned row0 = at.row * 128 + quarter * 32, limit = min(p.x.n, at.t0 + p.tile);
             float v[32];
+            if (p.split > 1)
+            {
+                // all blocks have been copied and multiplied: the stages are free
+                float *part = reinterpret_cast<float *>(stages) + quarter * 32 + lane;
+                const bool any = at.j < at.end;
+                if (any && !tc::barrier_wait(&sh.done[0], 0, &sh.gave_up)) break;
+                tc::fence_after();
+                for (unsigned c = first; c < p.tile; c += 64)
+                {
+                    if (any) tc::tensor_load32(tensor + c + (quarter * 32 << 16), v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) part[(c + i) * 128] = any ? v[i] : 0.f;
+                }
+                break;
+            }
             if (at.j == at.end)
             {
 #pragma unroll
@@ -243,6 +265,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
     }
 end:
     __syncwarp();
+    if (p.split > 1) // (all CTAs of the cluster come here, whatever became of their waits)
+    {
+        namespace cg = cooperative_groups;
+        const cg::cluster_group cluster = cg::this_cluster();
+        const float *part = reinterpret_cast<const float *>(stages);
+        cluster.sync();
+        const Steps at(p);
+        Y *y = reinterpret_cast<Y *>(p.y);
+        const unsigned rows = min(128u, p.a.n_rows - at.row * 128), columns = min(p.tile, p.x.n - at.t0);
+        for (unsigned i = threadIdx.x + kThreads * (blockIdx.x % p.split); i < columns * 32; i += kThreads * p.split)
+        {
+            float4 v[8]; // all on their way before the first is needed
+#pragma unroll
+            for (unsigned s = 0; s < 8; s++)
+                if (s < p.split) v[s] = *cluster.map_shared_rank(reinterpret_cast<const float4 *>(part) + i, s);
+            float sum[4] = {};
+#pragma unroll
+            for (unsigned s = 0; s < 8; s++)
+                if (s < p.split) sum[0] += v[s].x, sum[1] += v[s].y, sum[2] += v[s].z, sum[3] += v[s].w;
+            const unsigned r = i % 32 * 4;
+            Y *to = y + (uint64_t)(at.t0 + i / 32) * p.ldy + at.row * 128 + r;
+            if (p.pairs && sizeof(Y) == 2 && r + 4 <= rows)
+            {
+                Y four[4] = {from_float<Y>(sum[0]), from_float<Y>(sum[1]), from_float<Y>(sum[2]), from_float<Y>(sum[3])};
+                reinterpret_cast<unsigned *>(to)[0] = reinterpret_cast<const unsigned *>(four)[0], reinterpret_cast<unsigned *>(to)[1] = reinterpret_cast<const unsigned *>(four)[1];
+            }
+            else
+#pragma unroll
+                for (unsigned k = 0; k < 4; k++)
+                    if (r + k < rows) to[k] = from_float<Y>(sum[k]);
+        }
+        cluster.sync(); // (its shared memory is read until here)
+    }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -256,20 +311,21 @@ end:
     if (warp == 1) tc::tensor_free(tensor, 512);
 }
 
-// Rows of X a tile. The steps of a tile take as long as their products (2 clocks a row of X) or their copies do (some 50 bytes a clock and SM); a tile
-// costs some 2000 clocks beside its steps. Every size is looked at, for the waves that its tiles make of the SMs.
-unsigned tile_rows(const Block8Dev &a, unsigned n, int sm_count)
+// Rows of X a tile, and CTAs that share its blocks. A step takes as long as its 16 KB of A and its rows of X take to pass shared memory twice, at 128 bytes a
+// clock; a tile costs some 2500 clocks beside its steps, and as much again where sums of several CTAs are added up.
+void plan(const Block8Dev &a, unsigned n, int sm_count, unsigned *tile, unsigned *split)
 {
-    const double steps = (double)a.n_blocks / a.n_block_rows;
-    unsigned best = kMostRows;
     double least = 0;
     for (unsigned t = kMostRows; t >= 64; t -= 64)
-    {
-        const uint64_t tiles = (uint64_t)a.n_block_rows * ((n + t - 1) / t), waves = (tiles + sm_count - 1) / sm_count;
-        const double cost = waves * (2000.0 + steps * std::max(2.0 * t, (16384.0 + 128.0 * t) / 50.0));
-        if (t == kMostRows || cost < least) best = t, least = cost;
-    }
-    return best;
+        for (unsigned s = 1; s <= 8; s++)
+        {
+            const uint64_t tiles = (uint64_t)a.n_block_rows * ((n + t - 1) / t), waves = (tiles + sm_count - 1) / sm_count;
+            // (clusters find no room on the last SMs of a part of the chip)
+            if (s > 1 && (tiles * s * 10 > (uint64_t)sm_count * 9 || a.longest < 2 * s)) break;
+            const double steps = s > 1 ? (double)((a.longest + s - 1) / s) : (double)a.n_blocks / a.n_block_rows;
+            const double cost = waves * ((s > 1 ? 5000.0 : 2500.0) + steps * (16384 + 128.0 * t) / 64);
+            if ((t == kMostRows && s == 1) || cost < least) least = cost, *tile = t, *split = s;
+        }
 }
 
 template <class Y> cudaError_t product(const CUtensorMap &map_a, const CUtensorMap &map_x, const ProductArgs &p, int sm_count, cudaStream_t st)
@@ -278,7 +334,8 @@ template <class Y> cudaError_t product(const CUtensorMap &map_a, const CUtensorM
     static SharedAllowance allowance;
     const cudaError_t e = allowance.need((const void *)k_block8_product<Y>, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_block8_product<Y>, dim3(std::min<unsigned>(p.n_tiles, (unsigned)sm_count)), dim3(kThreads), smem, st, map_a, map_x, p);
+    const unsigned grid = p.split > 1 ? p.n_tiles * p.split : std::min<unsigned>(p.n_tiles, (unsigned)sm_count);
+    return launch_pdl_cluster(k_block8_product<Y>, p.split, dim3(grid), dim3(kThreads), smem, st, map_a, map_x, p);
 }
 } // namespace
 
@@ -287,7 +344,7 @@ cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const D
     if (x.n == 0) return cudaSuccess;
     ProductArgs p = {};
     p.a = a, p.x = x, p.y = y.p, p.ldy = y.ld, p.fault = fault;
-    p.tile = tile_rows(a, x.n, sm_count);
+    plan(a, x.n, sm_count, &p.tile, &p.split);
     p.tiles_x = (x.n + p.tile - 1) / p.tile;
     const uint64_t tiles = (uint64_t)a.n_block_rows * p.tiles_x;
     if (tiles > 0xf0000000u) return cudaErrorInvalidValue; // (2^38 rows of blocks' results and more)
