@@ -2,11 +2,11 @@
 #include "../../include/asp_b200.h"
 #include "block8.h"
 #include "block8_device.h"
+#include "host/block8_plan.hpp"
 #include "launch.h"
 
 #include <cooperative_groups.h>
 
-#include <algorithm>
 #include <type_traits>
 
 namespace asp
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(256) k_block8_get(const uint8_t *values, const
 
 // ---- products with a few rows ----------------------------------------------------------------------------------------
 
-// Y[t][128 R + r] = sum over the blocks j of block row R of 2^(kA + kX) sum over c of A_j[r][c] X_j[t][c].
+// n <= 32 rows. Y[t][128 R + r] = sum over the blocks j of block row R of 2^(kA + kX) sum over c of A_j[r][c] X_j[t][c].
 //
 // The matrix is read once and nothing else counts: 16 KB a block, four or five blocks ahead, as the A operand of m16n8k16 with a warp to 16 rows (a
 // thread copies what it will itself read: no warp waits for another's); X in shared memory is the B operand, 8 rows of it a tile. Both as fp16, which has every e4m3 number: the form for e4m3 converts
@@ -278,7 +278,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     FewShared<NT> &sh = *reinterpret_cast<FewShared<NT> *>(raw);
     const cg::cluster_group cluster = cg::this_cluster();
     const unsigned split = args.n_split, piece = blockIdx.x % split, br = args.a.order[blockIdx.x / split];
-    const unsigned t0 = blockIdx.y * 8 * NT, tokens = min(8u * NT, args.n - t0);
+    const unsigned tokens = args.n;
     const unsigned lo = args.a.ptr[br], len = args.a.ptr[br + 1] - lo;
     const unsigned j0 = lo + (unsigned)((uint64_t)len * piece / split), j1 = lo + (unsigned)((uint64_t)len * (piece + 1) / split);
     const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
@@ -326,7 +326,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
         }
     };
     // Until the kernels before this one are done the matrix may still be written: it is brought to L2, which is never behind, and read afterwards.
-    if (threadIdx.x == 0 && j0 < j1 && blockIdx.y == 0)
+    if (threadIdx.x == 0 && j0 < j1)
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(args.a.values + (uint64_t)j0 * 16384), "r"(min(j1 - j0, 8u) * 16384) : "memory");
     for (unsigned i = threadIdx.x; i < sizeof(sh.x) / 16; i += 256) reinterpret_cast<uint4 *>(sh.x)[i] = make_uint4(0, 0, 0, 0);
     for (unsigned i = threadIdx.x; i < 2 * 32; i += 256) (&sh.factor[0][0][0])[i] = make_float2(1.f, 1.f);
@@ -339,7 +339,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     unsigned block_scale = 127;
     const auto ask = [&](unsigned j) { // of the stage that begins with block j
         if (j + slot >= j1 || t >= tokens) return;
-        got.ask(args, t0 + t, args.a.col[j + slot], lane8);
+        got.ask(args, t, args.a.col[j + slot], lane8);
         block_scale = args.a.scales[j + slot];
     };
     const auto put = [&](unsigned j) {
@@ -385,7 +385,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
         for (unsigned s = 0; s < 8; s++) v[s] = s < split ? *cluster.map_shared_rank(&sh.part[t][r], s) : 0.f;
 #pragma unroll
         for (unsigned s = 0; s < 8; s++) sum += v[s]; // (in order; zeros behind the last change nothing)
-        if (br * 128 + r < args.a.n_rows) y[(uint64_t)(t0 + t) * args.ldy + br * 128 + r] = from_float<Y>(sum);
+        if (br * 128 + r < args.a.n_rows) y[(uint64_t)t * args.ldy + br * 128 + r] = from_float<Y>(sum);
     }
     cluster.sync(); // (its shared memory is read until here)
 }
@@ -397,7 +397,7 @@ template <int NT, class X, class Y> cudaError_t few(const FewArgs &args, cudaStr
     static SharedAllowance allowance;
     const cudaError_t e = allowance.need((const void *)kernel, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl_cluster(kernel, args.n_split, dim3(args.a.n_block_rows * args.n_split, (args.n + 8 * NT - 1) / (8 * NT)), dim3(256), smem, st, args);
+    return launch_pdl_cluster(kernel, args.n_split, dim3(args.a.n_block_rows * args.n_split), dim3(256), smem, st, args);
 }
 template <class X, class Y> cudaError_t few_by_rows(const FewArgs &args, cudaStream_t st)
 {
@@ -450,9 +450,7 @@ cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev
     args.n = n;
     args.y = y.p;
     args.ldy = y.ld;
-    const unsigned tiles = (n + 31) / 32;
-    // Two CTAs fit an SM, and all run at once: with twice as many as fit (8192 x 8192, one row, eight CTAs a block row) a call took 17.7 us instead of 13.2.
-    args.n_split = std::max(1u, std::min({8u, a.longest, 2u * sm_count / (a.n_block_rows * tiles)}));
+    args.n_split = host::block8_few_split(a.n_block_rows, a.longest, sm_count);
     return by_type(y.dtype, [&](auto ty) {
         using Y = decltype(ty);
         if (held)

@@ -4,6 +4,7 @@
 #include "../../include/asp_b200.h"
 #include "block8.h"
 #include "block8_device.h"
+#include "host/block8_plan.hpp"
 #include "launch.h"
 #include "tcgen05.h"
 #include "tensor_map.h"
@@ -28,7 +29,7 @@ using namespace block8;
 // result one after the other, each beginning with another part of it: the same order, and bits, every time.
 //
 // Warp 0 copies, warp 1 issues products, warps 4 to 11 and 12 to 19 unfold x, every second step each, and then store.
-constexpr unsigned kRows = 64;          // t a step
+constexpr unsigned kRows = host::kBlock8GradientRows; // t a step
 constexpr unsigned kTile = kRows * 128; // bytes of 64 columns of a step's rows in 16 bits, of 128 in 8
 constexpr unsigned kRoom = 8, kBlockBytes = 2 * kTile;        // dy: blocks of a step's rows, as many steps as fit
 constexpr unsigned kHeld = 4, kHeldBytes = kTile + 1024;      // x in 8 bits, and its scales
@@ -334,29 +335,6 @@ template <class Unfold> cudaError_t gradient(const CUtensorMap &map_dy, const CU
     return launch_pdl_cluster(k_block8_gradient<Unfold>, p.split, dim3(n_groups * p.split), dim3(kThreads), smem, st, map_dy, map_x, p);
 }
 
-// How many blocks a group has at most, and how many CTAs share its rows. Clocks of a step by what passes shared memory; a CTA takes some 8000 clocks beside its
-// steps and 2000 more for each block that it stores, and each further CTA of a cluster another 2000 for what it adds to. With more CTAs than SMs the last ones
-// end on average half a CTA's time after the others.
-void plan(const Block8Groups &g, unsigned steps, int sm_count, unsigned *most, unsigned *split)
-{
-    static const double clocks[4] = {640, 896, 1280, 1536};
-    double least = 0;
-    for (unsigned m = 1; m <= 4; m++)
-        for (unsigned s = 1; s <= 4; s *= 2)
-        {
-            if (s > steps) continue;
-            double all = 0, longest = 0;
-            for (unsigned k = 0; k < m; k++)
-            {
-                if (g.sizes[m - 1][k] == 0) continue;
-                const double one = 8000 + 2000.0 * (k + 1) + (s > 1 ? 2000.0 * (k + 1) : 0.0) + clocks[k] * ((steps + s - 1) / s);
-                all += one * g.sizes[m - 1][k] * s;
-                longest = one; // (larger k, longer)
-            }
-            const double time = g.count[m - 1] * s <= (unsigned)sm_count ? longest : std::max(longest, all / sm_count) + longest / 2;
-            if ((m == 1 && s == 1) || time < least) least = time, *most = m, *split = s;
-        }
-}
 } // namespace
 
 cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &groups, const Rows8Dev &x, const Dense &dy, float *out, bool accumulate, int sm_count, unsigned *fault, cudaStream_t st)
@@ -364,14 +342,15 @@ cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &group
     if (a.n_blocks == 0) return cudaSuccess;
     if (x.n == 0) return accumulate ? cudaSuccess : cudaMemsetAsync(out, 0, (size_t)a.n_blocks * 16384 * sizeof(float), st);
     GradientArgs p = {};
-    unsigned most = 1;
-    plan(groups, (x.n + kRows - 1) / kRows, sm_count, &most, &p.split);
+    const host::Block8GradientPlan plan = host::block8_gradient_plan(groups.sizes, x.n, sm_count);
+    const unsigned most = plan.most;
+    p.split = plan.split;
     p.groups = groups, p.x = x, p.list = groups.groups[most - 1];
     p.dy = dy.p, p.ld = dy.ld, p.out = out, p.accumulate = accumulate, p.fault = fault;
     p.n_rows = a.n_rows, p.n_cols = a.n_cols;
     p.stages = kRoom / most;
     p.columns = most == 1 ? 128 : most == 2 ? 256 : 512;
-    p.direct = ((uintptr_t)dy.p & 15) == 0 && dy.ld % 8 == 0;
+    p.direct = ((uintptr_t)dy.p & 15) == 0 && dy.ld % 8 == 0 && dy.ld < 1ull << 38; // (a tile map's distances are below 2^40 bytes)
     CUtensorMap map_dy, map_x;
     cudaError_t e = byte_map(&map_x, x.values, x.ld, x.n, x.ld, kRows, false); // as it lies, without swizzle
     if (e == cudaSuccess && p.direct)

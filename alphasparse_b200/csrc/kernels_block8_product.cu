@@ -6,6 +6,7 @@
 #include "../../include/asp_b200.h"
 #include "block8.h"
 #include "block8_device.h"
+#include "host/block8_plan.hpp"
 #include "launch.h"
 #include "tcgen05.h"
 #include "tensor_map.h"
@@ -31,7 +32,7 @@ using namespace block8;
 // some columns each.
 //
 // A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 9 store.
-constexpr unsigned kMostRows = 192;
+constexpr unsigned kMostRows = host::kBlock8ProductRows;
 constexpr unsigned kStages = 8; // at most
 constexpr unsigned kScaleBytes = 512 + 1024;
 constexpr unsigned kRoom = 221 * 1024; // of shared memory for stages
@@ -311,23 +312,6 @@ end:
     if (warp == 1) tc::tensor_free(tensor, 512);
 }
 
-// Rows of X a tile, and CTAs that share its blocks. A step takes as long as its 16 KB of A and its rows of X take to pass shared memory twice, at 128 bytes a
-// clock; a tile costs some 2500 clocks beside its steps, and as much again where sums of several CTAs are added up.
-void plan(const Block8Dev &a, unsigned n, int sm_count, unsigned *tile, unsigned *split)
-{
-    double least = 0;
-    for (unsigned t = kMostRows; t >= 64; t -= 64)
-        for (unsigned s = 1; s <= 8; s++)
-        {
-            const uint64_t tiles = (uint64_t)a.n_block_rows * ((n + t - 1) / t), waves = (tiles + sm_count - 1) / sm_count;
-            // (clusters find no room on the last SMs of a part of the chip)
-            if (s > 1 && (tiles * s * 10 > (uint64_t)sm_count * 9 || a.longest < 2 * s)) break;
-            const double steps = s > 1 ? (double)((a.longest + s - 1) / s) : (double)a.n_blocks / a.n_block_rows;
-            const double cost = waves * ((s > 1 ? 5000.0 : 2500.0) + steps * (16384 + 128.0 * t) / 64);
-            if ((t == kMostRows && s == 1) || cost < least) least = cost, *tile = t, *split = s;
-        }
-}
-
 template <class Y> cudaError_t product(const CUtensorMap &map_a, const CUtensorMap &map_x, const ProductArgs &p, int sm_count, cudaStream_t st)
 {
     const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
@@ -344,7 +328,8 @@ cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const D
     if (x.n == 0) return cudaSuccess;
     ProductArgs p = {};
     p.a = a, p.x = x, p.y = y.p, p.ldy = y.ld, p.fault = fault;
-    plan(a, x.n, sm_count, &p.tile, &p.split);
+    const host::Block8ProductPlan plan = host::block8_product_plan(a.n_block_rows, a.n_blocks, a.longest, x.n, sm_count);
+    p.tile = plan.tile, p.split = plan.split;
     p.tiles_x = (x.n + p.tile - 1) / p.tile;
     const uint64_t tiles = (uint64_t)a.n_block_rows * p.tiles_x;
     if (tiles > 0xf0000000u) return cudaErrorInvalidValue; // (2^38 rows of blocks' results and more)

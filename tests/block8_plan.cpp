@@ -1,0 +1,65 @@
+// The rules of csrc/host/block8_plan.cpp over sizes of all kinds: what they give is what the kernels take, and each variant is some call's.
+#include "../alphasparse_b200/csrc/host/block8_plan.cpp"
+
+#include <stdio.h>
+#include <stdlib.h>
+
+#include <set>
+#include <utility>
+
+using namespace asp::host;
+
+#define CHECK(c)                                           \
+    do                                                     \
+    {                                                      \
+        if (!(c))                                          \
+        {                                                  \
+            printf("line %d: %s\n", __LINE__, #c);         \
+            return 1;                                      \
+        }                                                  \
+    } while (0)
+
+int main()
+{
+    const int sms = 148;
+    std::set<unsigned> few;
+    std::set<std::pair<unsigned, unsigned>> products, gradients;
+    for (unsigned rows = 1; rows < 70000; rows = rows < 160 ? rows + 1 : rows * 3 / 2)
+        for (unsigned longest = 0; longest < 3000; longest = longest * 2 + 1)
+        {
+            const unsigned s = block8_few_split(rows, longest, sms);
+            CHECK(s >= 1 && s <= 8 && (s == 1 || s <= longest) && (s == 1 || rows * s <= 2u * sms));
+            few.insert(s);
+            for (unsigned n = 33; n < 100000; n = n * 3 / 2)
+            {
+                const Block8ProductPlan p = block8_product_plan(rows, (unsigned)(0.7 * rows * longest), longest, n, sms);
+                CHECK(p.tile % 64 == 0 && p.tile >= 64 && p.tile <= kBlock8ProductRows && p.split >= 1 && p.split <= 8);
+                // a CTA of a cluster has one tile, and all of them run at once
+                CHECK(p.split == 1 || ((unsigned long long)rows * ((n + p.tile - 1) / p.tile) * p.split <= (unsigned)sms && longest >= 2 * p.split));
+                products.insert({p.tile, p.split});
+            }
+        }
+    for (unsigned columns = 1; columns < 3000; columns = columns * 3 / 2 + 1)
+        for (unsigned each = 1; each <= 40; each++)
+        {
+            unsigned sizes[4][4] = {};
+            for (unsigned m = 1; m <= 4; m++)
+                for (unsigned k = 0, parts = (each + m - 1) / m; k < parts; k++) sizes[m - 1][each * (k + 1) / parts - each * k / parts - 1] += columns;
+            for (unsigned n = 1; n < 100000; n = n * 2 + 1)
+            {
+                const Block8GradientPlan p = block8_gradient_plan(sizes, n, sms);
+                CHECK(p.most >= 1 && p.most <= 4 && (p.split == 1 || p.split == 2 || p.split == 4));
+                CHECK(p.split <= (n + kBlock8GradientRows - 1) / kBlock8GradientRows); // each CTA has a step, so that its sums are there
+                gradients.insert({p.most, p.split});
+            }
+        }
+    const unsigned none[4][4] = {};
+    CHECK(block8_gradient_plan(none, 5, sms).most >= 1);
+    for (unsigned s : {1u, 2u, 4u, 8u}) CHECK(few.count(s));
+    for (unsigned t : {64u, 128u, 192u}) CHECK(products.count({t, 1}));
+    for (unsigned s : {2u, 4u, 8u}) CHECK(products.count({64, s}));
+    for (unsigned m = 1; m <= 4; m++) CHECK(gradients.count({m, 1}));
+    for (unsigned s : {2u, 4u}) CHECK(gradients.count({1, s}));
+    printf("%zu, %zu, %zu variants\n", few.size(), products.size(), gradients.size());
+    return 0;
+}

@@ -1,6 +1,8 @@
 """CPU suite: patterns of block-sparse 8-bit matrices and the refusals of their entry points, which come before any device is touched; the
 64-bit definition that the GPU tests compare with, against torch's own e4m3."""
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -109,3 +111,42 @@ def test_blocks_of_a_dense_matrix():
     assert s.shape == (3, 128, 128) and (s[1, :, 72:] == 0).all() and (s[2, 44:] == 0).all()
     back = ref.dense(p, (300, 200), s)
     assert torch.equal(back[:128], full[:128]) and (back[128:256] == 0).all() and (back[256:, :128] == 0).all() and torch.equal(back[256:, 128:], full[256:, 128:])
+
+
+def test_rules_on_sizes(tmp_path):
+    exe = str(tmp_path / "block8_plan")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", os.path.join(os.path.dirname(os.path.abspath(__file__)), "block8_plan.cpp"), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
+
+
+@pytest.mark.parametrize("args", [(0, None, 4, 0, 0, 0, 4, 0), (0, 0, 4, 0.0, 0, 0, 4, 0), (0, 0, 4, 0, 0, 0, 4), (0, 0, "f32", 0, 0, 0, 4, 0)])
+def test_apply_without_ctypes_takes_ints_only(args):
+    handle, matrix = C.c_void_p(), C.c_void_p()
+    call = capi._native().Apply(C.cast(block8._lib().asp_block8_apply, C.c_void_p).value, C.addressof(handle), C.addressof(matrix))
+    with pytest.raises(TypeError):
+        call(*args)
+    # handles are read at the call: a closed context or matrix is NULL to the library
+    assert call(0, 16, 4, 1, 0, 16, 4, 0) == 1 and capi.lib().asp_last_error() == b"NULL argument"
+
+
+def test_apply_with_and_without_the_binding(monkeypatch):
+    def matrix():
+        m = object.__new__(block8.Block8)
+        m.ctx = object.__new__(capi.Context)
+        m.ctx._h, m._h = C.c_void_p(), C.c_void_p()
+        m._apply = block8._bind_apply(m.ctx._h, m._h)
+        return m
+
+    def none():
+        raise ImportError
+
+    for _ in range(2):
+        m = matrix()
+        for x in (16, None, C.c_void_p(16)):
+            with pytest.raises(capi.AspError) as e:
+                m.apply(x, 1, "f32", 16, "f32")
+            assert e.value.status == 1
+        with pytest.raises(C.ArgumentError):
+            m.apply(1.5, 1, "f32", 16, "f32")
+        monkeypatch.setattr(capi, "_native", none)

@@ -320,6 +320,40 @@ def test_a_matrix_without_blocks_and_products_without_rows(asp_ctx, n):
     assert (y == 7.0).all()
 
 
+@pytest.mark.parametrize("n,n_rows,n_cols", [(64, 1024, 8192), (40, 4096, 2048), (700, 512, 512), (500, 2048, 1024), (2500, 1500, 1000)])
+def test_product_in_tiles_of_all_sizes(asp_ctx, n, n_rows, n_cols):
+    m, a = matrix(asp_ctx, 77, n_rows, n_cols, 0.8, transposed=False, empty_row=1)
+    x, held, y = rows(n, n, n_cols, "bf16"), Rows8(asp_ctx, n, n_cols), torch.empty(n, n_rows, device="cuda")
+    torch.cuda.synchronize()
+    held.quantize(x.data_ptr(), n, "bf16")
+    m.product(held, y.data_ptr(), "f32")
+    asp_ctx.synchronize()
+    assert_sums(y, ref.rows_in_8_bits(x), a, "f32", "tiles")
+    m.close()
+    held.close()
+
+
+@pytest.mark.parametrize("n", [7, 20, 100, 400])
+def test_rows_that_are_not_finite_keep_it_to_themselves(asp_ctx, n):
+    m, a = matrix(asp_ctx, 78, 700, 900, 1.0)
+    x = rows(2, n, 900, "f32")
+    x[1, 5], x[n // 2, 899] = float("nan"), float("inf")
+    held, y = Rows8(asp_ctx, n, 900), torch.empty(n, 700, device="cuda")
+    torch.cuda.synchronize()
+    held.quantize(x.data_ptr(), n, "f32")
+    for call in (lambda: m.product(held, y.data_ptr(), "f32"), lambda: m.apply(x.data_ptr(), min(n, 32), "f32", y.data_ptr(), "f32")):
+        y.fill_(7.0)
+        torch.cuda.synchronize()
+        call()
+        asp_ctx.synchronize()
+        bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+        bad[1] = bad[n // 2] = True
+        seen = n if (y[-1] != 7.0).any() else min(n, 32)
+        assert torch.equal(y[:seen].isnan().all(1), bad[:seen]) and torch.equal(y[:seen].isnan().any(1), bad[:seen])
+        good = ~bad[:seen]
+        assert_sums(y[:seen][good], ref.rows_in_8_bits(x)[:seen][good], a, "f32", "the other rows")
+
+
 @pytest.mark.parametrize("n", [4, 200])
 def test_scales_far_apart(asp_ctx, n):
     """Exponents whose sum no 32-bit number has, though the sums of products are ordinary; and rows of the largest numbers."""
@@ -378,6 +412,46 @@ def test_gradient(asp_ctx, n, n_rows, n_cols, density, dtype):
     assert ((out.double() - 2 * once).abs() <= size * (2 * (n + 1) * 2.0**-23) + once.abs() * 2.0**-22 + 2.0**-126).all()
     m.close()
     held.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("blocks,columns,n", [(1, 3, 1000), (1, 60, 400), (2, 100, 150), (3, 100, 70), (4, 100, 150), (5, 100, 130), (7, 40, 300)])
+def test_gradient_of_columns_of_blocks(asp_ctx, blocks, columns, n, dtype):
+    """Columns of 1 to 7 blocks, which are taken one to four together, by one CTA or a cluster that shares the rows."""
+    n_rows, n_cols = 128 * blocks - 3, 128 * columns - 5
+    p = pattern(1, n_rows, n_cols, 1.0)
+    m, held = Block8(asp_ctx, n_rows, n_cols, *p), Rows8(asp_ctx, n, n_cols)
+    g = gen(n)
+    x, dy = torch.randn(n, n_cols, generator=g, device="cuda").to(TYPES[dtype]), torch.randn(n, (n_rows + 7) // 8 * 8, generator=g, device="cuda").to(TYPES[dtype])
+    out = torch.full((m.n_blocks, 128, 128), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    held.quantize(x.data_ptr(), n, dtype)
+    m.gradient(held, dy.data_ptr(), dtype, out.data_ptr(), dy.stride(0))
+    asp_ctx.synchronize()
+    assert_gradient(out, dy[:, :n_rows], ref.rows_in_8_bits(x), p)
+    m.close()
+    held.close()
+
+
+def test_many_gradients_and_products_one_after_the_other(asp_ctx):
+    """Copies that overtake one another, warps ahead of others: 300 calls on a busy chip give the bits of the first."""
+    n = 4096
+    m, _ = matrix(asp_ctx, 6, 2048, 2048, 0.4)
+    x, dy = rows(1, n, 2048, "bf16"), rows(2, n, 2048, "bf16")
+    held, grads = Rows8(asp_ctx, n, 2048), Rows8(asp_ctx, n, 2048)
+    first = None
+    for k in range(6):
+        out = [torch.full((m.n_blocks, 128, 128), 7.0, device="cuda"), torch.full((n, 2048), 7.0, device="cuda"), torch.full((n, 2048), 7.0, device="cuda")]
+        torch.cuda.synchronize()
+        for _ in range(50):
+            held.quantize(x.data_ptr(), n, "bf16")
+            m.gradient(held, dy.data_ptr(), "bf16", out[0].data_ptr())
+            m.product(held, out[1].data_ptr(), "f32")
+            grads.quantize(dy.data_ptr(), n, "bf16")
+            m.product(grads, out[2].data_ptr(), "f32", transposed=True)
+        asp_ctx.synchronize()
+        first = first or out
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
 
 
 @pytest.mark.parametrize("pad,offset", [(1, 0), (8, 0), (0, 1), (7, 8)])
