@@ -65,8 +65,8 @@ struct Block8Groups
 {
     const unsigned *row, *col;   // of each block of A
     const unsigned *from;        // block of A^T -> block of A
-    const unsigned *groups[4];
-    unsigned count[4], sizes[4][4];
+    const unsigned *groups[2];
+    unsigned count[2], twos;
 };
 cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &groups, const Rows8Dev &x, const Dense &dy, float *out, bool accumulate, int sm_count, unsigned *fault, cudaStream_t st);
 } // namespace asp

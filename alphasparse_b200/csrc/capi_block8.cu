@@ -106,8 +106,8 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
         order[s] = take(p.side[s].order.size() * 4);
     }
     const Piece row = take(n * 4), place = take(n * 4), from = take(n * 4);
-    Piece groups[4];
-    for (int g = 0; g < 4; g++) groups[g] = take(p.groups[g].size() * 4);
+    Piece groups[2];
+    for (int g = 0; g < 2; g++) groups[g] = take(p.groups[g].size() * 4);
     std::vector<uint32_t> rows(n);
     for (uint32_t r = 0; r < p.side[0].rows(); r++) std::fill(rows.begin() + p.side[0].ptr[r], rows.begin() + p.side[0].ptr[r + 1], r);
     ASP_ON_DEVICE(ctx);
@@ -146,12 +146,12 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
     m->place = send(place, p.place.data());
     m->groups.row = m->row, m->groups.col = m->side[0].col;
     m->groups.from = send(from, p.from.data());
-    for (int g = 0; g < 4; g++)
+    for (int g = 0; g < 2; g++)
     {
         m->groups.groups[g] = send(groups[g], p.groups[g].data());
         m->groups.count[g] = (unsigned)p.groups[g].size();
-        std::copy(p.sizes[g], p.sizes[g] + 4, m->groups.sizes[g]);
     }
+    m->groups.twos = p.twos;
     e = ctx->stager.to_device(m->room.base, segments, ctx->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) return cuda_fail(e, "upload of the pattern");

@@ -66,21 +66,12 @@ asp_status make_pattern(u64 n_rows, u64 n_cols, const int64_t *block_ptr, const 
         }
     out.from.resize(n);
     for (u64 j = 0; j < n; j++) out.from[out.place[j]] = (u32)j;
-    for (u32 most = 1; most <= 4; most++)
-    {
-        std::vector<u32> &g = out.groups[most - 1];
-        for (u64 c = 0; c < nc; c++)
-        {
-            const u32 lo = t.ptr[c], len = t.ptr[c + 1] - lo, parts = (len + most - 1) / most;
-            for (u32 k = 0; k < parts; k++)
-            {
-                const u32 begin = (u32)((u64)len * k / parts), size = (u32)((u64)len * (k + 1) / parts) - begin;
-                g.push_back((lo + begin) | (size - 1) << 24);
-                out.sizes[most - 1][size - 1]++;
-            }
-        }
-        std::stable_sort(g.begin(), g.end(), [](u32 x, u32 y) { return x >> 24 > y >> 24; });
-    }
+    for (u32 i = 0; i < n; i++) out.groups[0].push_back(i);
+    for (u64 c = 0; c < nc; c++)
+        for (u32 i = t.ptr[c]; i + 1 < t.ptr[c + 1]; i += 2) out.groups[1].push_back(i | 1u << 31);
+    out.twos = (u32)out.groups[1].size();
+    for (u64 c = 0; c < nc; c++)
+        if ((t.ptr[c + 1] - t.ptr[c]) % 2) out.groups[1].push_back(t.ptr[c + 1] - 1);
     finish(a);
     finish(t);
     return ASP_OK;

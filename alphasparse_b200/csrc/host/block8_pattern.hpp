@@ -30,10 +30,9 @@ struct Block8Pattern
     Block8Side side[2];      // of A, of A^T
     std::vector<u32> place;  // where block i of A lies among the blocks of A^T
     std::vector<u32> from;   // the other way: which block of A is block i of A^T
-    // Blocks of A^T in groups of one block column of A and at most 1, 2, 3, 4 blocks, larger ones first: where the group begins, and in bits 24 and 25 how many
-    // there are less one. The columns' blocks are shared out evenly.
-    std::vector<u32> groups[4];
-    u32 sizes[4][4] = {}; // groups of 1 to 4 blocks among them
+    // Blocks of A^T one by one, and in twos of one block column of A, those that stay alone last: where the group begins, and in bit 31 whether there are two
+    std::vector<u32> groups[2];
+    u32 twos = 0; // groups of two blocks among the latter
     u64 blocks() const { return side[0].col.size(); }
 };
 

@@ -33,31 +33,21 @@ Block8ProductPlan block8_product_plan(unsigned n_block_rows, unsigned n_blocks, 
     return best;
 }
 
-// Clocks of a step by what passes shared memory; a CTA takes some 8000 clocks beside its steps and 2000 more for each block that it stores, and each
-// further CTA of a cluster another 2000 for what it adds to. With more CTAs than SMs the last ones end on average half a CTA's time after the others. Against all 12
-// choices on 8 shapes (300 to 8192 rows, 16 to 2048 blocks): within 15 % of the best, where the worst choice costs 2 to 10 times as much.
-Block8GradientPlan block8_gradient_plan(const unsigned sizes[4][4], unsigned n, int sm_count)
+// Clocks of a step by what passes shared memory; a call takes some 10000 clocks beside the steps of its longest CTA, and 3000 more for each CTA that adds to a block
+// that it shares (single blocks only: their sums stay in tensor memory).
+Block8GradientPlan block8_gradient_plan(unsigned blocks, unsigned twos, unsigned n, int sm_count)
 {
-    static const double clocks[4] = {640, 896, 1280, 1536};
     const unsigned steps = (unsigned)(((uint64_t)n + kBlock8GradientRows - 1) / kBlock8GradientRows);
+    const auto clocks = [&](uint64_t groups, double step) { return (groups + sm_count - 1) / sm_count * step * steps; };
     Block8GradientPlan best = {1, 1};
-    double least = -1;
-    for (unsigned m = 1; m <= 4; m++)
-        for (unsigned s = 1; s <= 4 && s <= steps; s *= 2)
-        {
-            double all = 0, longest = 0;
-            uint64_t groups = 0;
-            for (unsigned k = 0; k < m; k++)
-            {
-                if (sizes[m - 1][k] == 0) continue;
-                const double one = 8000 + 2000.0 * (k + 1) * (s > 1 ? 2 : 1) + clocks[k] * ((steps + s - 1) / s);
-                groups += sizes[m - 1][k];
-                all += one * sizes[m - 1][k] * s;
-                longest = one; // (of more blocks, longer)
-            }
-            const double time = groups * s <= (unsigned)sm_count ? longest : std::max(longest, all / sm_count) + longest / 2;
-            if (least < 0 || time < least) least = time, best = {m, s};
-        }
+    double least = clocks(blocks, 640);
+    if (twos && clocks(blocks - twos, 960) < least) least = clocks(blocks - twos, 960), best.most = 2; // (with what is added up by L2)
+    // (clusters find no room on the last SMs of a part of the chip)
+    for (unsigned s = 2; s <= 8 && s <= steps && (uint64_t)blocks * s * 10 <= (uint64_t)sm_count * 9; s *= 2)
+    {
+        const double time = 640.0 * ((steps + s - 1) / s) + 3000.0 * s;
+        if (time < least) least = time, best = {1, s};
+    }
     return best;
 }
 } // namespace host

@@ -18,14 +18,14 @@ struct Block8ProductPlan
 constexpr unsigned kBlock8ProductRows = 192;
 Block8ProductPlan block8_product_plan(unsigned n_block_rows, unsigned n_blocks, unsigned longest, unsigned n, int sm_count);
 
-// Gradients (k_block8_gradient): blocks of a block column that share x at most (1 to 4), and CTAs that share the rows of a group (1, 2, 4).
-// sizes[m - 1][k - 1]: groups of k blocks where groups have m at most.
+// Gradients (k_block8_gradient): blocks of a block column that share x at most (1, 2), and CTAs that share the rows of a group (1, 2, 4, 8).
+// blocks: stored ones; twos: groups of two where there are two at most.
 struct Block8GradientPlan
 {
     unsigned most, split;
 };
 constexpr unsigned kBlock8GradientRows = 64; // rows a step
-Block8GradientPlan block8_gradient_plan(const unsigned sizes[4][4], unsigned n, int sm_count);
+Block8GradientPlan block8_gradient_plan(unsigned blocks, unsigned twos, unsigned n, int sm_count);
 } // namespace host
 } // namespace asp
 #endif

@@ -24,12 +24,17 @@ using namespace block8;
 // tcgen05.mma takes as it is (columns of k). D's lanes are c, so that a warp stores 128 bytes in a row of a block.
 //
 // What bounds it is shared memory, 128 bytes a clock and SM: for 64 rows t, x of a block column passes it four times (8 KB in, 8 out, unfolded 16 in and
-// with each product 16 out), dy of a block row twice and more. So up to four blocks of a column share x: 48 KB a block instead of 80 for
-// one alone, 384 clocks where the products take 256. Groups of blocks go to CTAs, and where there are few of them a cluster shares the rows t; its CTAs add to the
-// result one after the other, each beginning with another part of it: the same order, and bits, every time.
+// with each product 16 out), dy of a block row twice and more. Two blocks of a column share x: 56 KB a block instead of 80 for one alone, 448 clocks
+// where the products take 256. (Four would be 384, but leave no room for a second D: measured the same, with the rows below in one sum.)
 //
-// Warp 0 copies, warp 1 issues products, warps 4 to 11 and 12 to 19 unfold x, every second step each, and then store.
+// Tensor cores cut off what they add up to, which over 8192 rows in one sum showed as 6.5e-6 of the result, where sums that are rounded have 6e-7. So D takes
+// 1280 rows (7e-7), then another one the next, while the first is added, rounded, to the sum of those before: in tensor memory where a
+// group is one block, by L2 where it is two (12 % of the time for 8192 rows). A CTA per SM goes through the groups. Where there are few of them a cluster shares the
+// rows of one; its CTAs then add to the result one after the other, each beginning with another part of it: the same order, and bits, every time.
+//
+// Warp 0 copies, warp 1 issues products, warps 4 to 11 add up and store, warps 12 to 19 and 20 to 27 unfold x, every second step each.
 constexpr unsigned kRows = host::kBlock8GradientRows; // t a step
+constexpr unsigned kRound = 1280 / kRows;             // steps a sum
 constexpr unsigned kTile = kRows * 128; // bytes of 64 columns of a step's rows in 16 bits, of 128 in 8
 constexpr unsigned kRoom = 8, kBlockBytes = 2 * kTile;        // dy: blocks of a step's rows, as many steps as fit
 constexpr unsigned kHeld = 4, kHeldBytes = kTile + 1024;      // x in 8 bits, and its scales
@@ -37,20 +42,20 @@ constexpr unsigned kHeld = 4, kHeldBytes = kTile + 1024;      // x in 8 bits, an
 // copies to a place before the first has arrived (they may overtake one another), and take the one before both, of the same parity, for it.
 static_assert(kHeld % 2 == 0, "places for x are shared out between two groups of warps");
 constexpr unsigned kUnfolded = 3, kUnfoldedBytes = 2 * kTile; // x in 16 bits: 64 columns after 64 columns, a row t 128 bytes
-constexpr unsigned kThreads = 640;
+constexpr unsigned kThreads = 896;
 
 struct GradientArgs
 {
     Block8Groups groups;
     Rows8Dev x;
     const unsigned *list; // groups of blocks
+    unsigned n_groups, most;
     const void *dy;
     uint64_t ld;
     float *out;
     unsigned n_rows, n_cols;
     unsigned split;  // CTAs that share the rows of a group
     unsigned stages; // of dy
-    unsigned columns; // of tensor memory
     bool direct; // dy can be copied by tiles
     bool accumulate;
     unsigned *fault;
@@ -58,7 +63,7 @@ struct GradientArgs
 
 struct Shared
 {
-    uint64_t full[kRoom], empty[kRoom], held[kHeld], read[kHeld], unfolded[kUnfolded], used[kUnfolded], done;
+    uint64_t full[kRoom], empty[kRoom], held[kHeld], read[kHeld], unfolded[kUnfolded], used[kUnfolded], done[2], taken[2];
     unsigned tensor, gave_up;
 };
 
@@ -117,6 +122,44 @@ struct UnfoldB16
 // the column of a block that D's lane has
 template <class Unfold> __device__ __forceinline__ unsigned column_of(unsigned lane) { return Unfold::bf16 && (lane % 4 == 1 || lane % 4 == 2) ? lane ^ 3 : lane; }
 
+// Where a lane's part of a group's blocks goes: looked up once a group, as each look-up waits for the one before
+struct Places
+{
+    float *to[2];     // element (0, c) of each block
+    unsigned rows[2]; // of them inside the matrix; 0: the column is not
+};
+template <class Unfold> __device__ __forceinline__ Places places(const GradientArgs &p, unsigned group, unsigned quarter, unsigned lane)
+{
+    const unsigned first = group & 0x7fffffffu, c = quarter * 32 + column_of<Unfold>(lane);
+    Places at = {};
+#pragma unroll
+    for (unsigned k = 0; k < 2; k++)
+        if (k == 0 || group >> 31)
+        {
+            const unsigned b = p.groups.from[first + k];
+            at.to[k] = p.out + (uint64_t)b * 16384 + c;
+            at.rows[k] = p.groups.col[b] * 128 + c < p.n_cols ? min(128u, p.n_rows - p.groups.row[b] * 128) : 0;
+        }
+    return at;
+}
+// 16 columns of D (r, block after block) from c on, a quarter of its lanes
+__device__ __forceinline__ void store_columns(const Places &at, const float *v, unsigned c, bool add)
+{
+    const unsigned r0 = c % 128, rows = c < 128 ? at.rows[0] : at.rows[1];
+    float *to = (c < 128 ? at.to[0] : at.to[1]) + r0 * 128;
+    if (add)
+    {
+#pragma unroll
+        for (unsigned k = 0; k < 16; k++) // (by L2, without waiting; one thread's additions to a place stay in order)
+            if (r0 + k < rows) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to + k * 128), "f"(v[k]) : "memory");
+    }
+    else
+    {
+#pragma unroll
+        for (unsigned k = 0; k < 16; k++) __stcg(to + k * 128, r0 + k < rows ? v[k] : 0.f); // zero outside the matrix
+    }
+}
+
 template <class Unfold>
 __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ GradientArgs p)
 {
@@ -126,9 +169,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
     unsigned char *dys = raw + (1024 - tc::shared_address(raw) % 1024) % 1024;
     unsigned char *halves = dys + kRoom * kBlockBytes, *bytes = halves + kUnfolded * kUnfoldedBytes;
     const unsigned warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-    const unsigned piece = blockIdx.x % p.split, group = p.list[blockIdx.x / p.split], first = group & 0xffffffu, blocks = 1 + (group >> 24);
+    const unsigned piece = blockIdx.x % p.split, u0 = blockIdx.x / p.split, stride = gridDim.x / p.split;
     const unsigned steps = (p.x.n + kRows - 1) / kRows, step0 = (unsigned)((uint64_t)steps * piece / p.split), step1 = (unsigned)((uint64_t)steps * (piece + 1) / p.split);
-    const unsigned col = p.groups.col[p.groups.from[first]];
+    const unsigned width_d = p.most * 128; // two Ds, and the sum of a single block behind them
     if (threadIdx.x == 32)
     {
         tc::prefetch_map(&map_x);
@@ -139,11 +182,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         for (unsigned i = 0; i < p.stages; i++) tc::barrier_init(&sh.full[i], 1), tc::barrier_init(&sh.empty[i], 1);
         for (unsigned i = 0; i < kHeld; i++) tc::barrier_init(&sh.held[i], 1), tc::barrier_init(&sh.read[i], 8);
         for (unsigned i = 0; i < kUnfolded; i++) tc::barrier_init(&sh.unfolded[i], 8), tc::barrier_init(&sh.used[i], 1);
-        tc::barrier_init(&sh.done, 1);
+        for (unsigned i = 0; i < 2; i++) tc::barrier_init(&sh.done[i], 1), tc::barrier_init(&sh.taken[i], 8);
         sh.gave_up = 0;
         tc::fence_barrier_init();
     }
-    if (warp == 1) tc::tensor_alloc(&sh.tensor, p.columns);
+    if (warp == 1) tc::tensor_alloc(&sh.tensor, 512);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -156,30 +199,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         if (tc::one_lane())
         {
             unsigned s = 0, phase = 0, x = 0, x_phase = 0;
-            unsigned r[4];
-#pragma unroll
-            for (unsigned k = 0; k < 4; k++) r[k] = k < blocks ? p.groups.row[p.groups.from[first + k]] * 128 : 0;
-            for (unsigned i = step0; i < step1; i++)
+            for (unsigned u = u0; u < p.n_groups; u += stride)
             {
-                const int t = (int)(i * kRows);
-                if (!tc::barrier_wait(&sh.read[x], x_phase ^ 1, &sh.gave_up)) goto end;
-                unsigned char *to = bytes + x * kHeldBytes;
-                tc::barrier_expect(&sh.held[x], kTile + 512);
-                tc::copy_tile(to, &map_x, (int)(col * 128), t, &sh.held[x]);
-                tc::copy_bytes(to + kTile, p.x.scales + ((uint64_t)(col / 4) * p.x.pieces + t / 128) * 512, 512, &sh.held[x]);
-                if (++x == kHeld) x = 0, x_phase ^= 1;
-                if (!p.direct) continue;
-                if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
-                tc::barrier_expect(&sh.full[s], blocks * kBlockBytes);
-                to = dys + s * blocks * kBlockBytes;
+                const unsigned first = p.list[u] & 0x7fffffffu, blocks = 1 + (p.list[u] >> 31), col = p.groups.col[p.groups.from[first]];
+                const unsigned r[2] = {p.groups.row[p.groups.from[first]] * 128, blocks > 1 ? p.groups.row[p.groups.from[first + 1]] * 128 : 0};
+                for (unsigned i = step0; i < step1; i++)
+                {
+                    const int t = (int)(i * kRows);
+                    if (!tc::barrier_wait(&sh.read[x], x_phase ^ 1, &sh.gave_up)) goto end;
+                    unsigned char *to = bytes + x * kHeldBytes;
+                    tc::barrier_expect(&sh.held[x], kTile + 512);
+                    tc::copy_tile(to, &map_x, (int)(col * 128), t, &sh.held[x]);
+                    tc::copy_bytes(to + kTile, p.x.scales + ((uint64_t)(col / 4) * p.x.pieces + t / 128) * 512, 512, &sh.held[x]);
+                    if (++x == kHeld) x = 0, x_phase ^= 1;
+                    if (!p.direct) continue;
+                    if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
+                    tc::barrier_expect(&sh.full[s], blocks * kBlockBytes);
+                    to = dys + s * p.most * kBlockBytes;
 #pragma unroll
-                for (unsigned k = 0; k < 4; k++)
-                    if (k < blocks)
-                    {
-                        tc::copy_tile(to + k * kBlockBytes, &map_dy, (int)r[k], t, &sh.full[s]);
-                        tc::copy_tile(to + k * kBlockBytes + kTile, &map_dy, (int)r[k] + 64, t, &sh.full[s]);
-                    }
-                if (++s == p.stages) s = 0, phase ^= 1;
+                    for (unsigned k = 0; k < 2; k++)
+                        if (k < blocks)
+                        {
+                            tc::copy_tile(to + k * kBlockBytes, &map_dy, (int)r[k], t, &sh.full[s]);
+                            tc::copy_tile(to + k * kBlockBytes + kTile, &map_dy, (int)r[k] + 64, t, &sh.full[s]);
+                        }
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
             }
         }
     }
@@ -187,131 +232,172 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
     {
         if (tc::one_lane())
         {
-            const unsigned wide = tc::halves(256, Unfold::bf16), narrow = tc::halves(128, Unfold::bf16);
-            unsigned s = 0, phase = 0, h = 0, h_phase = 0;
-            for (unsigned i = step0; i < step1; i++)
+            unsigned s = 0, phase = 0, h = 0, h_phase = 0, d = 0, d_phase = 0;
+            for (unsigned u = u0; u < p.n_groups; u += stride)
             {
-                if (p.direct && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
-                if (!tc::barrier_wait(&sh.unfolded[h], h_phase, &sh.gave_up)) goto end;
-                tc::fence_after();
-                const unsigned x = tc::shared_address(halves + h * kUnfoldedBytes);
-                for (unsigned b = 0; b < blocks; b += 2)
+                const unsigned shape = tc::halves(128 + 128 * (p.list[u] >> 31), Unfold::bf16);
+                for (unsigned i = step0, left = 0; i < step1; i++)
                 {
-                    const unsigned dy = tc::shared_address(dys + (s * blocks + b) * kBlockBytes), shape = b + 1 < blocks ? wide : narrow;
+                    const bool fresh = left == 0;
+                    if (fresh)
+                    {
+                        if (!tc::barrier_wait(&sh.taken[d], d_phase ^ 1, &sh.gave_up)) goto end;
+                        left = kRound;
+                    }
+                    if (p.direct && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
+                    if (!tc::barrier_wait(&sh.unfolded[h], h_phase, &sh.gave_up)) goto end;
+                    tc::fence_after();
+                    const unsigned x = tc::shared_address(halves + h * kUnfoldedBytes), dy = tc::shared_address(dys + s * p.most * kBlockBytes);
 #pragma unroll
                     for (unsigned k = 0; k < kRows / 16; k++) // 16 rows of 128 bytes on
-                        tc::mma_halves(tensor + b * 128, tc::columns_of_k(x + 2048 * k, kTile), tc::columns_of_k(dy + 2048 * k, kTile), shape, i > step0 || k > 0);
+                        tc::mma_halves(tensor + d * width_d, tc::columns_of_k(x + 2048 * k, kTile), tc::columns_of_k(dy + 2048 * k, kTile), shape, !fresh || k > 0);
+                    tc::commit(&sh.empty[s]);
+                    tc::commit(&sh.used[h]);
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                    if (++h == kUnfolded) h = 0, h_phase ^= 1;
+                    if (--left == 0 || i + 1 == step1)
+                    {
+                        tc::commit(&sh.done[d]);
+                        left = 0;
+                        d ^= 1;
+                        if (d == 0) d_phase ^= 1;
+                    }
                 }
-                tc::commit(&sh.empty[s]);
-                tc::commit(&sh.used[h]);
+            }
+        }
+    }
+    else if (warp >= 12)
+    {
+        // 8 lanes and 16 columns a lane to a row t: 4 rows a warp at once, warp w rows 4 w on, then 32 rows further
+        const unsigned lane8 = lane % 8, w = (warp - 12) % 8, row0 = w * 4 + lane / 8, mine = (warp - 12) / 8;
+        unsigned s = 0, phase = 0, x = 0, x_phase = 0, h = 0, h_phase = 0, turn = 0;
+        for (unsigned u = u0; u < p.n_groups; u += stride)
+        {
+            const unsigned first = p.list[u] & 0x7fffffffu, blocks = 1 + (p.list[u] >> 31), byte = p.groups.col[p.groups.from[first]] % 4;
+            for (unsigned i = step0; i < step1; i++)
+            {
+                if (turn == mine)
+                {
+                    if (!tc::barrier_wait(&sh.held[x], x_phase, &sh.gave_up)) goto end;
+                    const unsigned char *from = bytes + x * kHeldBytes;
+                    uint4 q[2];
+                    unsigned scale[2];
+#pragma unroll
+                    for (unsigned j = 0; j < 2; j++)
+                    {
+                        const unsigned t = row0 + 32 * j, row = i * kRows + t;
+                        q[j] = *reinterpret_cast<const uint4 *>(from + t * 128 + 16 * lane8);
+                        scale[j] = row < p.x.n ? from[kTile + row0 * 16 + row / 32 % 4 * 4 + byte] : 127; // (rows behind the last one are zeros, with any scale)
+                    }
+                    // The next copy may come while these are unfolded. Reads and copies are of different proxies: without the fence a copy overtook reads that
+                    // other kernels' warps held up.
+                    tc::fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) tc::barrier_arrive(&sh.read[x]);
+                    if (!tc::barrier_wait(&sh.used[h], h_phase ^ 1, &sh.gave_up)) goto end;
+                    unsigned char *to = halves + h * kUnfoldedBytes + lane8 / 4 * kTile;
+#pragma unroll
+                    for (unsigned j = 0; j < 2; j++)
+                    {
+                        const unsigned t = row0 + 32 * j;
+                        unsigned v[8];
+                        Unfold::words(q[j], scale[j], v);
+                        // 16-byte pieces 2 l and 2 l + 1 of the row's 128 bytes, swapped in the second half so that eight lanes meet no conflict
+                        unsigned char *line = to + t * 128;
+                        const unsigned at = lane8 % 4 * 2, second = lane8 / 4;
+                        const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
+                        *reinterpret_cast<uint4 *>(line + (((at + second) ^ (t % 8)) * 16)) = second ? hi : lo;
+                        *reinterpret_cast<uint4 *>(line + (((at + 1 - second) ^ (t % 8)) * 16)) = second ? lo : hi;
+                    }
+                    if (!p.direct) // dy element by element, into the same swizzle
+                    {
+                        if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
+                        const unsigned short *dy = reinterpret_cast<const unsigned short *>(p.dy);
+                        for (unsigned k = 0; k < blocks; k++)
+                        {
+                            const unsigned r0 = p.groups.row[p.groups.from[first + k]] * 128;
+                            for (unsigned e = w * 32 + lane; e < kRows * 128; e += 256)
+                            {
+                                const unsigned t = e / 128, r = e % 128;
+                                const unsigned short v = i * kRows + t < p.x.n && r0 + r < p.n_rows ? dy[(uint64_t)(i * kRows + t) * p.ld + r0 + r] : 0;
+                                *reinterpret_cast<unsigned short *>(dys + (s * p.most + k) * kBlockBytes + r / 64 * kTile + t * 128 + ((r % 64 / 8) ^ (t % 8)) * 16 + r % 8 * 2) = v;
+                            }
+                        }
+                    }
+                    tc::fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) tc::barrier_arrive(&sh.unfolded[h]);
+                }
+                turn ^= 1;
                 if (++s == p.stages) s = 0, phase ^= 1;
+                if (++x == kHeld) x = 0, x_phase ^= 1;
                 if (++h == kUnfolded) h = 0, h_phase ^= 1;
             }
-            tc::commit(&sh.done);
         }
     }
     else if (warp >= 4)
     {
-        // 8 lanes and 16 columns a lane to a row t: 4 rows a warp at once, warp w rows 4 w on, then 32 rows further
-        const unsigned lane8 = lane % 8, w = (warp - 4) % 8, row0 = w * 4 + lane / 8, mine = (warp - 4) / 8, byte = col % 4;
-        unsigned s = 0, phase = 0, x = 0, x_phase = 0, h = 0, h_phase = 0, turn = 0;
-        for (unsigned i = step0; i < step1; i++)
+        // two warps to a quarter of D's lanes, every second 16 columns each
+        unsigned d = 0, d_phase = 0;
+        const unsigned quarter = warp % 4, mine = (warp - 4) / 4 * 16;
+        for (unsigned u = u0; u < p.n_groups; u += stride)
         {
-            if (turn == mine)
+            const unsigned blocks = 1 + (p.list[u] >> 31);
+            const Places at = places<Unfold>(p, p.list[u], quarter, lane);
+            for (unsigned i = step0; i < step1; i += kRound)
             {
-                if (!tc::barrier_wait(&sh.held[x], x_phase, &sh.gave_up)) goto end;
-                const unsigned char *from = bytes + x * kHeldBytes;
-                uint4 q[2];
-                unsigned scale[2];
-#pragma unroll
-                for (unsigned j = 0; j < 2; j++)
+                if (!tc::barrier_wait<64>(&sh.done[d], d_phase, &sh.gave_up)) goto end;
+                tc::fence_after();
+                const bool last = i + kRound >= step1 && p.split == 1;
+                for (unsigned c = mine; c < blocks * 128; c += 32)
                 {
-                    const unsigned t = row0 + 32 * j, row = i * kRows + t;
-                    q[j] = *reinterpret_cast<const uint4 *>(from + t * 128 + 16 * lane8);
-                    scale[j] = row < p.x.n ? from[kTile + row0 * 16 + row / 32 % 4 * 4 + byte] : 127; // (rows behind the last one are zeros, with any scale)
-                }
-                __syncwarp();
-                if (lane == 0) tc::barrier_arrive(&sh.read[x]); // the next copy may come while these are unfolded
-                if (!tc::barrier_wait(&sh.used[h], h_phase ^ 1, &sh.gave_up)) goto end;
-                unsigned char *to = halves + h * kUnfoldedBytes + lane8 / 4 * kTile;
-#pragma unroll
-                for (unsigned j = 0; j < 2; j++)
-                {
-                    const unsigned t = row0 + 32 * j;
-                    unsigned v[8];
-                    Unfold::words(q[j], scale[j], v);
-                    // 16-byte pieces 2 l and 2 l + 1 of the row's 128 bytes, swapped in the second half so that eight lanes meet no conflict
-                    unsigned char *line = to + t * 128;
-                    const unsigned at = lane8 % 4 * 2, second = lane8 / 4;
-                    const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
-                    *reinterpret_cast<uint4 *>(line + (((at + second) ^ (t % 8)) * 16)) = second ? hi : lo;
-                    *reinterpret_cast<uint4 *>(line + (((at + 1 - second) ^ (t % 8)) * 16)) = second ? lo : hi;
-                }
-                if (!p.direct) // dy element by element, into the same swizzle
-                {
-                    if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
-                    const unsigned short *dy = reinterpret_cast<const unsigned short *>(p.dy);
-                    for (unsigned k = 0; k < blocks; k++)
+                    float v[16];
+                    tc::tensor_load16(tensor + d * width_d + c + (quarter * 32 << 16), v);
+                    if (p.most == 2) store_columns(at, v, c, p.accumulate || i > step0);
+                    else
                     {
-                        const unsigned r0 = p.groups.row[p.groups.from[first + k]] * 128;
-                        for (unsigned e = w * 32 + lane; e < kRows * 128; e += 256)
+                        const unsigned sum = tensor + 256 + c + (quarter * 32 << 16);
+                        if (i > step0)
                         {
-                            const unsigned t = e / 128, r = e % 128;
-                            const unsigned short v = i * kRows + t < p.x.n && r0 + r < p.n_rows ? dy[(uint64_t)(i * kRows + t) * p.ld + r0 + r] : 0;
-                            *reinterpret_cast<unsigned short *>(dys + (s * blocks + k) * kBlockBytes + r / 64 * kTile + t * 128 + ((r % 64 / 8) ^ (t % 8)) * 16 + r % 8 * 2) = v;
+                            float o[16];
+                            tc::tensor_load16(sum, o);
+#pragma unroll
+                            for (int k = 0; k < 16; k++) v[k] += o[k];
                         }
+                        if (last) store_columns(at, v, c, p.accumulate);
+                        else tc::tensor_store16(sum, v);
                     }
                 }
-                tc::fence_async_shared();
+                tc::fence_before();
                 __syncwarp();
-                if (lane == 0) tc::barrier_arrive(&sh.unfolded[h]);
+                if (lane == 0) tc::barrier_arrive(&sh.taken[d]);
+                d ^= 1;
+                if (d == 0) d_phase ^= 1;
             }
-            turn ^= 1;
-            if (++s == p.stages) s = 0, phase ^= 1;
-            if (++x == kHeld) x = 0, x_phase ^= 1;
-            if (++h == kUnfolded) h = 0, h_phase ^= 1;
         }
-        if (!tc::barrier_wait<64>(&sh.done, 0, &sh.gave_up)) goto end;
     }
 end:
     __syncwarp();
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    // The columns of D (r, block after block) in `split` parts, a multiple of 32 columns each: this CTA begins with its own. (All CTAs of the cluster go through
-    // this together, whatever became of their waits.)
-    for (unsigned turn = 0; turn < p.split; turn++)
+    // A cluster (and a block each): the sum's columns in `split` parts of 16 to 64; a CTA begins with its own. (All CTAs of the cluster go through this
+    // together, whatever became of their waits.)
+    if (p.split > 1)
     {
-        const unsigned part = (piece + turn) % p.split, width = blocks * 128 / p.split;
-        if (warp >= 4 && !sh.gave_up)
+        const Places at = places<Unfold>(p, p.list[u0], warp % 4, lane);
+        const unsigned width = 128 / p.split;
+        for (unsigned turn = 0; turn < p.split; turn++)
         {
-            // four warps to a quarter of D's lanes
-            const unsigned quarter = warp % 4, c = quarter * 32 + column_of<Unfold>(lane);
-            const bool inside = col * 128 + c < p.n_cols;
-            for (unsigned d = part * width + (warp - 4) / 4 * 32; d < (part + 1) * width; d += 128)
+            const unsigned part = (piece + turn) % p.split, c = part * width + (warp - 4) / 4 * 16;
+            if (warp >= 4 && c < (part + 1) * width && !sh.gave_up)
             {
-                float v[32], o[32];
-                const unsigned b = p.groups.from[first + d / 128], r0 = d % 128, rows = p.n_rows - p.groups.row[b] * 128;
-                float *to = p.out + (uint64_t)b * 16384 + r0 * 128 + c;
-                if (p.accumulate || turn > 0) // (all of them on their way before the first is needed)
-                {
-#pragma unroll
-                    for (unsigned k = 0; k < 32; k++) o[k] = __ldcg(to + k * 128);
-                }
-                tc::tensor_load32(tensor + d + (quarter * 32 << 16), v);
-                if (p.accumulate || turn > 0)
-                {
-#pragma unroll
-                    for (unsigned k = 0; k < 32; k++) __stcg(to + k * 128, (inside && r0 + k < rows ? v[k] : 0.f) + o[k]); // zero outside the matrix
-                }
-                else
-                {
-#pragma unroll
-                    for (unsigned k = 0; k < 32; k++) __stcg(to + k * 128, inside && r0 + k < rows ? v[k] : 0.f);
-                }
+                float v[16];
+                tc::tensor_load16(tensor + 256 + c + (warp % 4 * 32 << 16), v);
+                store_columns(at, v, c, p.accumulate || turn > 0);
             }
+            cg::this_cluster().sync();
         }
-        if (p.split > 1) cg::this_cluster().sync();
     }
     tc::fence_before();
     __syncthreads();
@@ -323,16 +409,17 @@ end:
         while (tc::now_ns() - since < 10000000ull) __nanosleep(1000);
         if (threadIdx.x == 0 && p.fault) *reinterpret_cast<volatile unsigned *>(p.fault) = 1;
     }
-    if (warp == 1) tc::tensor_free(tensor, p.columns);
+    if (warp == 1) tc::tensor_free(tensor, 512);
 }
 
-template <class Unfold> cudaError_t gradient(const CUtensorMap &map_dy, const CUtensorMap &map_x, const GradientArgs &p, unsigned n_groups, cudaStream_t st)
+template <class Unfold> cudaError_t gradient(const CUtensorMap &map_dy, const CUtensorMap &map_x, const GradientArgs &p, int sm_count, cudaStream_t st)
 {
     const size_t smem = kRoom * kBlockBytes + kUnfolded * kUnfoldedBytes + kHeld * kHeldBytes + 1024;
     static SharedAllowance allowance;
     const cudaError_t e = allowance.need((const void *)k_block8_gradient<Unfold>, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl_cluster(k_block8_gradient<Unfold>, p.split, dim3(n_groups * p.split), dim3(kThreads), smem, st, map_dy, map_x, p);
+    const unsigned grid = p.split > 1 ? p.n_groups * p.split : std::min<unsigned>(p.n_groups, (unsigned)sm_count);
+    return launch_pdl_cluster(k_block8_gradient<Unfold>, p.split, dim3(grid), dim3(kThreads), smem, st, map_dy, map_x, p);
 }
 
 } // namespace
@@ -342,14 +429,12 @@ cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &group
     if (a.n_blocks == 0) return cudaSuccess;
     if (x.n == 0) return accumulate ? cudaSuccess : cudaMemsetAsync(out, 0, (size_t)a.n_blocks * 16384 * sizeof(float), st);
     GradientArgs p = {};
-    const host::Block8GradientPlan plan = host::block8_gradient_plan(groups.sizes, x.n, sm_count);
-    const unsigned most = plan.most;
-    p.split = plan.split;
-    p.groups = groups, p.x = x, p.list = groups.groups[most - 1];
+    const host::Block8GradientPlan plan = host::block8_gradient_plan(a.n_blocks, groups.twos, x.n, sm_count);
+    p.most = plan.most, p.split = plan.split;
+    p.groups = groups, p.x = x, p.list = groups.groups[p.most - 1], p.n_groups = groups.count[p.most - 1];
     p.dy = dy.p, p.ld = dy.ld, p.out = out, p.accumulate = accumulate, p.fault = fault;
     p.n_rows = a.n_rows, p.n_cols = a.n_cols;
-    p.stages = kRoom / most;
-    p.columns = most == 1 ? 128 : most == 2 ? 256 : 512;
+    p.stages = kRoom / p.most;
     p.direct = ((uintptr_t)dy.p & 15) == 0 && dy.ld % 8 == 0 && dy.ld < 1ull << 38; // (a tile map's distances are below 2^40 bytes)
     CUtensorMap map_dy, map_x;
     cudaError_t e = byte_map(&map_x, x.values, x.ld, x.n, x.ld, kRows, false); // as it lies, without swizzle
@@ -357,7 +442,7 @@ cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &group
         e = tensor_map(&map_dy, dy.dtype == ASP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dy.p, a.n_rows, x.n, dy.ld * 2, 64, kRows);
     else map_dy = map_x; // (not used)
     if (e != cudaSuccess) return e;
-    if (dy.dtype == ASP_BF16) return gradient<UnfoldB16>(map_dy, map_x, p, groups.count[most - 1], st);
-    return gradient<Unfold16>(map_dy, map_x, p, groups.count[most - 1], st);
+    if (dy.dtype == ASP_BF16) return gradient<UnfoldB16>(map_dy, map_x, p, sm_count, st);
+    return gradient<Unfold16>(map_dy, map_x, p, sm_count, st);
 }
 } // namespace asp

@@ -42,24 +42,20 @@ int main()
     for (unsigned columns = 1; columns < 3000; columns = columns * 3 / 2 + 1)
         for (unsigned each = 1; each <= 40; each++)
         {
-            unsigned sizes[4][4] = {};
-            for (unsigned m = 1; m <= 4; m++)
-                for (unsigned k = 0, parts = (each + m - 1) / m; k < parts; k++) sizes[m - 1][each * (k + 1) / parts - each * k / parts - 1] += columns;
             for (unsigned n = 1; n < 100000; n = n * 2 + 1)
             {
-                const Block8GradientPlan p = block8_gradient_plan(sizes, n, sms);
-                CHECK(p.most >= 1 && p.most <= 4 && (p.split == 1 || p.split == 2 || p.split == 4));
+                const Block8GradientPlan p = block8_gradient_plan(columns * each, columns * (each / 2), n, sms);
+                CHECK((p.most == 1 || (p.most == 2 && each > 1)) && (p.split == 1 || p.split == 2 || p.split == 4 || p.split == 8));
                 CHECK(p.split <= (n + kBlock8GradientRows - 1) / kBlock8GradientRows); // each CTA has a step, so that its sums are there
+                CHECK(p.split == 1 || (p.most == 1 && columns * each * p.split <= (unsigned)sms));
                 gradients.insert({p.most, p.split});
             }
         }
-    const unsigned none[4][4] = {};
-    CHECK(block8_gradient_plan(none, 5, sms).most >= 1);
     for (unsigned s : {1u, 2u, 4u, 8u}) CHECK(few.count(s));
     for (unsigned t : {64u, 128u, 192u}) CHECK(products.count({t, 1}));
     for (unsigned s : {2u, 4u, 8u}) CHECK(products.count({64, s}));
-    for (unsigned m = 1; m <= 4; m++) CHECK(gradients.count({m, 1}));
-    for (unsigned s : {2u, 4u}) CHECK(gradients.count({1, s}));
+    for (unsigned s : {1u, 2u, 4u, 8u}) CHECK(gradients.count({1, s}));
+    CHECK(gradients.count({2, 1}));
     printf("%zu, %zu, %zu variants\n", few.size(), products.size(), gradients.size());
     return 0;
 }

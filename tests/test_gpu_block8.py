@@ -415,9 +415,9 @@ def test_gradient(asp_ctx, n, n_rows, n_cols, density, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("blocks,columns,n", [(1, 3, 1000), (1, 60, 400), (2, 100, 150), (3, 100, 70), (4, 100, 150), (5, 100, 130), (7, 40, 300)])
+@pytest.mark.parametrize("blocks,columns,n", [(1, 3, 1000), (1, 60, 400), (2, 100, 150), (3, 100, 70), (4, 100, 150), (5, 100, 130), (7, 40, 300), (2, 80, 5000), (1, 150, 4500), (2, 2, 9000)])
 def test_gradient_of_columns_of_blocks(asp_ctx, blocks, columns, n, dtype):
-    """Columns of 1 to 7 blocks, which are taken one to four together, by one CTA or a cluster that shares the rows."""
+    """Columns of 1 to 7 blocks, which are taken one by one or in twos, by one CTA or a cluster that shares the rows, in sums of 2048 rows."""
     n_rows, n_cols = 128 * blocks - 3, 128 * columns - 5
     p = pattern(1, n_rows, n_cols, 1.0)
     m, held = Block8(asp_ctx, n_rows, n_cols, *p), Rows8(asp_ctx, n, n_cols)
