@@ -61,42 +61,99 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// The 16 elements that lane `lane8` of 8 has of a row's block of 128 columns, and what becomes of them. vec: the row begins on a 16-byte
-// boundary and has the whole block; the lane then has pieces of 16 bytes, every eighth one, and otherwise every eighth element, so that the lanes read and
-// write side by side either way.
-template <class T> __device__ __forceinline__ unsigned column_in_block(int i, unsigned lane8, bool vec)
+// ---- copies to shared memory of 16 bytes, by the thread that will read them ----
+__device__ __forceinline__ void copy16(void *to, const void *from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_are_one_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n> __device__ __forceinline__ void wait_for_all_groups_but() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
+
+// ---- rows that begin anywhere ----
+// A row's elements are taken 16 bytes at a time whether it begins on a 16-byte boundary or not: a lane loads the aligned piece in which its own begins,
+// gets the next one from the lane beside it and shifts the two. (Loads and stores element by element took 2.4 and 3 times as long for rows of
+// 4001 bf16.) A piece that is not all inside the caller's matrix is put together from the elements that are.
+
+// bytes [o, o + 16) of `a` and `b` side by side; o = 4 * words + bits / 8
+__device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, unsigned words, unsigned bits)
+{
+    unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 7; i++) w[i] = words & 1 ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; i++) w[i] = words & 2 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 shuffled(uint4 v, unsigned from)
+{
+    return make_uint4(__shfl_sync(~0u, v.x, from), __shfl_sync(~0u, v.y, from), __shfl_sync(~0u, v.z, from), __shfl_sync(~0u, v.w, from));
+}
+// the 16 bytes at p (on a 16-byte boundary), those of them that are in [lo, hi); T: what lies there
+template <class T> __device__ __forceinline__ uint4 load_piece(uintptr_t p, uintptr_t lo, uintptr_t hi)
+{
+    if (p >= lo && p + 16 <= hi) return *reinterpret_cast<const uint4 *>(p);
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (p + 16 <= lo || p >= hi) return r;
+    T e[16 / sizeof(T)];
+#pragma unroll
+    for (unsigned i = 0; i < 16 / sizeof(T); i++)
+    {
+        const uintptr_t at = p + i * sizeof(T);
+        e[i] = at >= lo && at < hi ? *reinterpret_cast<const T *>(at) : from_float<T>(0.f);
+    }
+    memcpy(&r, e, 16);
+    return r;
+}
+
+// The 16 elements that lane `lane8` of 8 has of a row's block of 128 columns: pieces of 16 bytes, every eighth one.
+template <class T> __device__ __forceinline__ unsigned column_in_block(int i, unsigned lane8)
 {
     constexpr int per = 16 / sizeof(T);
-    return vec ? i / per * 8 * per + lane8 * per + i % per : 8 * i + lane8;
+    return i / per * 8 * per + lane8 * per + i % per;
 }
-// as they lie in memory, zeros behind the row's end
+// as they come from memory, from where a block begins (`first`) and with what is inside [lo, hi)
 template <class T> struct Raw
 {
-    uint4 w[sizeof(T)];
-    __device__ __forceinline__ void load(const T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec)
+    static constexpr int per = 16 / sizeof(T), pieces = 16 / per;
+    uint4 w[pieces], more; // more: the piece behind the block's last, of its last lane
+    unsigned words, bits;
+    __device__ __forceinline__ void load(const T *first, const T *lo, const T *hi, unsigned lane8)
     {
-        constexpr int per = 16 / sizeof(T);
-        if (vec)
+        const uintptr_t o = (uintptr_t)first & 15, at = (uintptr_t)first - o + 16 * lane8;
+        words = (unsigned)o / 4, bits = (unsigned)o % 4 * 8;
 #pragma unroll
-            for (int i = 0; i < 16 / per; i++) w[i] = *reinterpret_cast<const uint4 *>(row + col0 + column_in_block<T>(i * per, lane8, true));
-        else
-        {
-            T e[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-            {
-                const unsigned c = col0 + 8 * i + lane8;
-                e[i] = c < n_cols ? row[c] : from_float<T>(0.f);
-            }
-            memcpy(w, e, sizeof(w));
-        }
+        for (int i = 0; i < pieces; i++) w[i] = load_piece<T>(at + 128 * i, (uintptr_t)lo, (uintptr_t)hi);
+        if (o && lane8 == 7) more = load_piece<T>(at + 128 * (pieces - 1) + 16, (uintptr_t)lo, (uintptr_t)hi);
     }
-    __device__ __forceinline__ void floats(float *v) const
+    // all lanes of the warp take part; `columns` of the block are in the row, zeros behind them
+    __device__ __forceinline__ void floats(float *v, unsigned lane8, unsigned columns) const
     {
+        uint4 u[pieces];
+        const unsigned lane = threadIdx.x % 32, beside = lane8 < 7 ? lane + 1 : lane - 7;
+        if (__any_sync(~0u, words | bits))
+        {
+#pragma unroll
+            for (int i = 0; i < pieces; i++)
+            {
+                // the first lane of a block is asked for its next piece, by the last one
+                uint4 next = shuffled(lane8 == 0 && i + 1 < pieces ? w[i + 1 < pieces ? i + 1 : i] : w[i], beside);
+                if (i + 1 == pieces && lane8 == 7) next = more;
+                u[i] = shifted(w[i], next, words, bits);
+            }
+        }
+        else
+#pragma unroll
+            for (int i = 0; i < pieces; i++) u[i] = w[i];
         T e[16];
-        memcpy(e, w, sizeof(w));
+        memcpy(e, u, sizeof(u));
 #pragma unroll
         for (int i = 0; i < 16; i++) v[i] = to_float(e[i]);
+        if (columns < 128)
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (column_in_block<T>(i, lane8) >= columns) v[i] = 0.f;
     }
 };
 // The scale of what the eight lanes of a block have, and whether something infinite is among it. All lanes of the warp take part. (fmaxf passes NaN over;
@@ -127,46 +184,65 @@ __device__ __forceinline__ void pack16(const float *v, unsigned scale, bool infi
     for (int i = 0; i < 4; i++) q[i] = infinite ? pack4<true>(v + 4 * i, inv) : pack4<false>(v + 4 * i, inv);
 }
 // and to where they belong; `to` is the block's first byte
-template <class T> __device__ __forceinline__ void store_block(const unsigned *q, bool vec, unsigned lane8, uint8_t *to)
+template <class T> __device__ __forceinline__ void store_block(const unsigned *q, unsigned lane8, uint8_t *to)
 {
     constexpr int per = 16 / sizeof(T);
-    if (vec)
 #pragma unroll
-        for (int i = 0; i < 16; i += per)
-        {
-            uint8_t *at = to + column_in_block<T>(i, lane8, true);
-            if constexpr (per == 4) *reinterpret_cast<unsigned *>(at) = q[i / 4];
-            else *reinterpret_cast<uint2 *>(at) = make_uint2(q[i / 4], q[i / 4 + 1]);
-        }
-    else
-#pragma unroll
-        for (int i = 0; i < 16; i++) to[8 * i + lane8] = (uint8_t)(q[i / 4] >> 8 * (i % 4));
+    for (int i = 0; i < 16; i += per)
+    {
+        uint8_t *at = to + column_in_block<T>(i, lane8);
+        if constexpr (per == 4) *reinterpret_cast<unsigned *>(at) = q[i / 4];
+        else *reinterpret_cast<uint2 *>(at) = make_uint2(q[i / 4], q[i / 4 + 1]);
+    }
 }
-// the other way: a block in 8 bits to the caller's type
-template <class T> __device__ __forceinline__ void restore_block(const uint8_t *from, float scale, T *row, unsigned col0, unsigned n_cols, unsigned lane8, bool vec)
+// The other way, for a warp's four blocks: `from` is the block's first byte, `first` where it goes to, `end` where the row ends. Pieces of 16 bytes that are not all
+// the warp's are stored element by element. All lanes of the warp take part.
+template <class T> __device__ __forceinline__ void restore_block(const uint8_t *from, float scale, T *first, T *end, unsigned lane8)
 {
-    constexpr int per = 16 / sizeof(T);
-    if (vec)
+    constexpr int per = 16 / sizeof(T), pieces = 16 / per;
+    const unsigned lane = threadIdx.x % 32;
+    uint4 u[pieces];
 #pragma unroll
-        for (int i = 0; i < 16; i += per)
+    for (int i = 0; i < pieces; i++)
+    {
+        const unsigned c = column_in_block<T>(i * per, lane8);
+        float v[per];
+#pragma unroll
+        for (int k = 0; k < per; k += 4) unpack4(*reinterpret_cast<const unsigned *>(from + c + k), v + k);
+        T e[per];
+#pragma unroll
+        for (int k = 0; k < per; k++) e[k] = from_float<T>(v[k] * scale);
+        memcpy(&u[i], e, 16);
+    }
+    const uintptr_t o = (uintptr_t)first & 15, lo = (uintptr_t)(first - lane / 8 * 128), hi = min((uintptr_t)end, lo + 512 * sizeof(T)); // of the warp's elements
+    const auto put = [&](uintptr_t at, uint4 w) {
+        if (at >= lo && at + 16 <= hi) *reinterpret_cast<uint4 *>(at) = w;
+        else
         {
-            const unsigned c = column_in_block<T>(i, lane8, true);
-            float v[per];
+            T e[per];
+            memcpy(e, &w, 16);
 #pragma unroll
-            for (int k = 0; k < per; k += 4) unpack4(*reinterpret_cast<const unsigned *>(from + c + k), v + k);
-            uint4 w;
-            T *e = reinterpret_cast<T *>(&w);
-#pragma unroll
-            for (int k = 0; k < per; k++) e[k] = from_float<T>(v[k] * scale);
-            *reinterpret_cast<uint4 *>(row + col0 + c) = w;
+            for (int k = 0; k < per; k++)
+                if (at + k * sizeof(T) >= lo && at + k * sizeof(T) < hi) *reinterpret_cast<T *>(at + k * sizeof(T)) = e[k];
         }
-    else
+    };
+    uintptr_t at = (uintptr_t)first - o + 16 * lane8;
+    if (o == 0) // (of a row: the same for all of the warp)
+    {
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-        {
-            const unsigned c = 8 * i + lane8;
-            if (col0 + c < n_cols) row[col0 + c] = from_float<T>(__low2float(unpack2(from[c])) * scale);
-        }
+        for (int i = 0; i < pieces; i++) put(at + 128 * i, u[i]);
+        return;
+    }
+    // the last o bytes of the piece before, and the first of one's own
+    const unsigned words = (16 - (unsigned)o) / 4, bits = (16 - (unsigned)o) % 4 * 8;
+#pragma unroll
+    for (int i = 0; i < pieces; i++)
+    {
+        const uint4 beside = shuffled(u[i], lane - 1 & 31), far = shuffled(u[i > 0 ? i - 1 : pieces - 1], i > 0 ? lane + 7 & 31 : lane - 1 & 31);
+        put(at + 128 * i, shifted(lane8 ? beside : far, u[i], words, bits));
+    }
+    // behind the warp's last piece
+    if (lane == 31) put(at + 128 * (pieces - 1) + 16, shifted(u[pieces - 1], make_uint4(0, 0, 0, 0), words, bits));
 }
 } // namespace block8
 } // namespace asp

@@ -21,29 +21,27 @@ template <class F> cudaError_t by_type(int dtype, F f)
     if (dtype == ASP_F16) return f(__half());
     return f(__nv_bfloat16());
 }
-template <class T> bool vectors(const Dense &x) { return ((uintptr_t)x.p & 15) == 0 && (x.ld * sizeof(T)) % 16 == 0; }
 
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
 // A row's four blocks to a warp, 8 lanes and 16 elements a lane each, so that an element is read once, its block's largest is known after
 // three exchanges, and the four scales leave as a word. Bounded by memory. Eight rows to a CTA: no warp waits for another.
-template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const T *x, uint64_t ld, bool vec, unsigned n, Rows8Dev out)
+template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const T *x, uint64_t ld, unsigned n, Rows8Dev out)
 {
     const unsigned lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (out.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
     const unsigned blk0 = blockIdx.x % fours * 4, blk = blk0 + lane / 8, row = blockIdx.x / fours * 8 + threadIdx.x / 32;
     grid_wait();
     grid_release();
     if (row >= n) return;
-    const bool together = vec && (blk + 1) * 128 <= out.n_cols;
     Raw<T> raw;
-    raw.load(x + (uint64_t)row * ld, blk * 128, out.n_cols, lane8, together); // (zeros behind the last block)
+    raw.load(x + (uint64_t)row * ld + blk * 128, x, x + (uint64_t)(n - 1) * ld + out.n_cols, lane8);
     float v[16];
-    raw.floats(v);
+    raw.floats(v, lane8, out.n_cols - min(out.n_cols, blk * 128)); // (zeros behind the last column, and behind the last block)
     bool infinite;
     const unsigned scale = scale_of_8(v, infinite);
     unsigned q[4];
     pack16(v, scale, infinite, q);
-    if (blk < n_blocks) store_block<T>(q, together, lane8, out.values + (uint64_t)row * out.ld + blk * 128);
+    if (blk < n_blocks) store_block<T>(q, lane8, out.values + (uint64_t)row * out.ld + blk * 128);
     unsigned four = scale << lane / 8 * 8;
     four |= __shfl_xor_sync(~0u, four, 8);
     four |= __shfl_xor_sync(~0u, four, 16);
@@ -51,14 +49,16 @@ template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const
 }
 
 // the same the other way
-template <class T> __global__ void __launch_bounds__(256) k_rows8_restore(Rows8Dev x, T *out, uint64_t ld, bool vec)
+template <class T> __global__ void __launch_bounds__(256) k_rows8_restore(Rows8Dev x, T *out, uint64_t ld)
 {
     const unsigned lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (x.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
     const unsigned blk = blockIdx.x % fours * 4 + lane / 8, row = blockIdx.x / fours * 8 + threadIdx.x / 32;
     grid_wait();
     grid_release();
-    if (row >= x.n || blk >= n_blocks) return;
-    restore_block(x.values + (uint64_t)row * x.ld + blk * 128, power(x.scales[scale_at(x, row, blk)]), out + (uint64_t)row * ld, blk * 128, x.n_cols, lane8, vec && (blk + 1) * 128 <= x.n_cols);
+    if (row >= x.n) return;
+    T *to = out + (uint64_t)row * ld;
+    const unsigned b = min(blk, n_blocks - 1); // (lanes without a block read the last one's, and store nothing)
+    restore_block(x.values + (uint64_t)row * x.ld + b * 128, power(x.scales[scale_at(x, row, b)]), to + blk * 128, to + x.n_cols, lane8);
 }
 
 // ---- the matrix's values --------------------------------------------------------------------------------------------
@@ -186,15 +186,8 @@ struct FewArgs
     void *y;
     uint64_t ldx, ldy;
     unsigned n, n_split;
-    bool vec;
 };
 
-__device__ __forceinline__ void copy16(void *to, const void *from)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_are_one_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int n> __device__ __forceinline__ void wait_for_all_groups_but() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
 __device__ __forceinline__ void mma_f16(float *c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
 {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -220,16 +213,17 @@ struct Held // X is in 8 bits already
 template <class X> struct Fetched
 {
     Raw<X> raw;
-    bool vec;
+    unsigned columns; // of the block that are in the row
     __device__ __forceinline__ void ask(const FewArgs &args, uint64_t row, unsigned kb, unsigned lane8)
     {
-        vec = args.vec && (kb + 1) * 128 <= args.a.n_cols;
-        raw.load(reinterpret_cast<const X *>(args.x) + row * args.ldx, kb * 128, args.a.n_cols, lane8, vec);
+        const X *x = reinterpret_cast<const X *>(args.x);
+        columns = args.a.n_cols - kb * 128;
+        raw.load(x + row * args.ldx + kb * 128, x, x + (args.n - 1) * args.ldx + args.a.n_cols, lane8);
     }
     __device__ __forceinline__ unsigned put(uint8_t *to, unsigned lane8, bool there) const // (`there` or not, for the exchanges)
     {
         float v[16];
-        raw.floats(v);
+        raw.floats(v, lane8, columns);
         bool infinite;
         const unsigned scale = scale_of_8(v, infinite);
         unsigned q[4], h[8];
@@ -237,17 +231,13 @@ template <class X> struct Fetched
         unpack16(make_uint4(q[0], q[1], q[2], q[3]), h);
         if (!there) return scale;
         constexpr int per = 16 / sizeof(X);
-        if (vec)
 #pragma unroll
-            for (int i = 0; i < 16; i += per)
-            {
-                uint8_t *at = to + 2 * column_in_block<X>(i, lane8, true);
-                if constexpr (per == 4) *reinterpret_cast<uint2 *>(at) = make_uint2(h[i / 2], h[i / 2 + 1]);
-                else *reinterpret_cast<uint4 *>(at) = make_uint4(h[i / 2], h[i / 2 + 1], h[i / 2 + 2], h[i / 2 + 3]);
-            }
-        else
-#pragma unroll
-            for (int i = 0; i < 16; i++) *reinterpret_cast<unsigned short *>(to + 2 * (8 * i + lane8)) = (unsigned short)(h[i / 2] >> 16 * (i % 2));
+        for (int i = 0; i < 16; i += per)
+        {
+            uint8_t *at = to + 2 * column_in_block<X>(i, lane8);
+            if constexpr (per == 4) *reinterpret_cast<uint2 *>(at) = make_uint2(h[i / 2], h[i / 2 + 1]);
+            else *reinterpret_cast<uint4 *>(at) = make_uint4(h[i / 2], h[i / 2 + 1], h[i / 2 + 2], h[i / 2 + 3]);
+        }
         return scale;
     }
 };
@@ -413,7 +403,7 @@ cudaError_t launch_rows8_quantize(const Dense &x, unsigned n, const Rows8Dev &ou
     return by_type(x.dtype, [&](auto t) {
         using T = decltype(t);
         const unsigned grid = (out.n_cols + 511) / 512 * ((n + 7) / 8);
-        return launch_pdl(k_rows8_quantize<T>, dim3(grid), dim3(256), 0, st, (const T *)x.p, x.ld, vectors<T>(x), n, out);
+        return launch_pdl(k_rows8_quantize<T>, dim3(grid), dim3(256), 0, st, (const T *)x.p, x.ld, n, out);
     });
 }
 
@@ -423,7 +413,7 @@ cudaError_t launch_rows8_restore(const Rows8Dev &x, const Dense &out, cudaStream
     return by_type(out.dtype, [&](auto t) {
         using T = decltype(t);
         const unsigned grid = (x.n_cols + 511) / 512 * ((x.n + 7) / 8);
-        return launch_pdl(k_rows8_restore<T>, dim3(grid), dim3(256), 0, st, x, (T *)out.p, out.ld, vectors<T>(out));
+        return launch_pdl(k_rows8_restore<T>, dim3(grid), dim3(256), 0, st, x, (T *)out.p, out.ld);
     });
 }
 
@@ -462,7 +452,6 @@ cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev
         args.ldx = x->ld;
         return by_type(x->dtype, [&](auto tx) {
             using X = decltype(tx);
-            args.vec = vectors<X>(*x);
             return few_by_rows<X, Y>(args, st);
         });
     });

@@ -43,6 +43,11 @@ constexpr unsigned kHeld = 4, kHeldBytes = kTile + 1024;      // x in 8 bits, an
 static_assert(kHeld % 2 == 0, "places for x are shared out between two groups of warps");
 constexpr unsigned kUnfolded = 3, kUnfoldedBytes = 2 * kTile; // x in 16 bits: 64 columns after 64 columns, a row t 128 bytes
 constexpr unsigned kThreads = 896;
+// Rows of dy that are not all on 16-byte boundaries cannot be copied by tiles. The warps that unfold x bring them, one of their steps ahead, in the aligned
+// pieces of 16 bytes that they lie in, and shift them to where they belong: twice as long for a step as by tiles (element by element it was
+// 17 times). They then take a part of dy's room, and groups are single blocks.
+constexpr unsigned kPitch = 272, kRawBytes = kRows * kPitch, kShiftedStages = 3; // 17 pieces a row
+static_assert(kShiftedStages * kBlockBytes + 4 * kRawBytes <= kRoom * kBlockBytes, "two steps of each group of warps beside the stages");
 
 struct GradientArgs
 {
@@ -270,7 +275,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
     {
         // 8 lanes and 16 columns a lane to a row t: 4 rows a warp at once, warp w rows 4 w on, then 32 rows further
         const unsigned lane8 = lane % 8, w = (warp - 12) % 8, row0 = w * 4 + lane / 8, mine = (warp - 12) / 8;
-        unsigned s = 0, phase = 0, x = 0, x_phase = 0, h = 0, h_phase = 0, turn = 0;
+        unsigned s = 0, phase = 0, x = 0, x_phase = 0, h = 0, h_phase = 0, turn = 0, parity = 0;
+        // rows of dy that begin anywhere
+        unsigned char *raws = dys + kShiftedStages * kBlockBytes + mine * 2 * kRawBytes;
+        const auto offset_of = [&](unsigned t, unsigned r0) { return (unsigned)((uintptr_t)p.dy + ((uint64_t)t * p.ld + r0) * 2) & 15u; };
+        const auto settle = [&](unsigned &u, unsigned &i) { // step i of the rows, or as much further on in the groups after this one
+            while (u < p.n_groups && i >= step1) i -= step1 - step0, u += stride;
+        };
+        const auto ask = [&](unsigned u, unsigned i, unsigned to) {
+            if (u < p.n_groups)
+            {
+                const unsigned r0 = p.groups.row[p.groups.from[p.list[u] & 0x7fffffffu]] * 128, j = lane % 16;
+                const uintptr_t lo = (uintptr_t)p.dy, hi = lo + ((uint64_t)(p.x.n - 1) * p.ld + p.n_rows) * 2;
+#pragma unroll
+                for (unsigned k = 0; k < 4; k++)
+                {
+                    const unsigned row = 16 * k + 2 * w + lane / 16, t = i * kRows + row;
+                    const uintptr_t at = lo + ((uint64_t)t * p.ld + r0) * 2 - offset_of(t, r0) + 16 * j;
+                    uint4 *piece = reinterpret_cast<uint4 *>(raws + to * kRawBytes + row * kPitch) + j;
+                    const auto bring = [&](uint4 *piece, uintptr_t at) {
+                        if (t < p.x.n && at >= lo && at + 16 <= hi) copy16(piece, reinterpret_cast<const void *>(at));
+                        else *piece = t < p.x.n ? load_piece<__half>(at, lo, hi) : make_uint4(0, 0, 0, 0);
+                    };
+                    bring(piece, at);
+                    if (j == 15) bring(piece + 1, at + 16);
+                }
+            }
+            copies_are_one_group();
+        };
+        if (!p.direct)
+        {
+            unsigned first_u = u0, first_i = step0 + mine;
+            settle(first_u, first_i);
+            ask(first_u, first_i, 0);
+        }
         for (unsigned u = u0; u < p.n_groups; u += stride)
         {
             const unsigned first = p.list[u] & 0x7fffffffu, blocks = 1 + (p.list[u] >> 31), byte = p.groups.col[p.groups.from[first]] % 4;
@@ -309,20 +347,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                         *reinterpret_cast<uint4 *>(line + (((at + second) ^ (t % 8)) * 16)) = second ? hi : lo;
                         *reinterpret_cast<uint4 *>(line + (((at + 1 - second) ^ (t % 8)) * 16)) = second ? lo : hi;
                     }
-                    if (!p.direct) // dy element by element, into the same swizzle
+                    if (!p.direct)
                     {
+                        unsigned next_u = u, next_i = i + 2;
+                        settle(next_u, next_i);
+                        __syncwarp(); // (the lanes beside have read what is copied to)
+                        ask(next_u, next_i, parity ^ 1);
+                        wait_for_all_groups_but<1>();
+                        __syncwarp();
                         if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
-                        const unsigned short *dy = reinterpret_cast<const unsigned short *>(p.dy);
-                        for (unsigned k = 0; k < blocks; k++)
+                        const unsigned r0 = p.groups.row[p.groups.from[first]] * 128, j = lane % 16;
+                        const int columns = (int)(p.n_rows - r0) - (int)(8 * j); // of the piece, that are in the matrix
+#pragma unroll
+                        for (unsigned k = 0; k < 4; k++)
                         {
-                            const unsigned r0 = p.groups.row[p.groups.from[first + k]] * 128;
-                            for (unsigned e = w * 32 + lane; e < kRows * 128; e += 256)
+                            const unsigned t = 16 * k + 2 * w + lane / 16, o = offset_of(i * kRows + t, r0);
+                            const uint4 *piece = reinterpret_cast<const uint4 *>(raws + parity * kRawBytes + t * kPitch) + j;
+                            uint4 v = shifted(piece[0], piece[1], o / 4, o % 4 * 8);
+                            if (columns < 8)
                             {
-                                const unsigned t = e / 128, r = e % 128;
-                                const unsigned short v = i * kRows + t < p.x.n && r0 + r < p.n_rows ? dy[(uint64_t)(i * kRows + t) * p.ld + r0 + r] : 0;
-                                *reinterpret_cast<unsigned short *>(dys + (s * p.most + k) * kBlockBytes + r / 64 * kTile + t * 128 + ((r % 64 / 8) ^ (t % 8)) * 16 + r % 8 * 2) = v;
+                                const auto keep = [&](unsigned word, int e) { return columns > e + 1 ? word : columns > e ? word & 0xffffu : 0u; };
+                                v = make_uint4(keep(v.x, 0), keep(v.y, 2), keep(v.z, 4), keep(v.w, 6));
                             }
+                            *reinterpret_cast<uint4 *>(dys + s * kBlockBytes + j / 8 * kTile + t * 128 + ((j % 8) ^ (t % 8)) * 16) = v;
                         }
+                        parity ^= 1;
                     }
                     tc::fence_async_shared();
                     __syncwarp();
@@ -429,13 +478,14 @@ cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &group
     if (a.n_blocks == 0) return cudaSuccess;
     if (x.n == 0) return accumulate ? cudaSuccess : cudaMemsetAsync(out, 0, (size_t)a.n_blocks * 16384 * sizeof(float), st);
     GradientArgs p = {};
-    const host::Block8GradientPlan plan = host::block8_gradient_plan(a.n_blocks, groups.twos, x.n, sm_count);
+    const bool direct = ((uintptr_t)dy.p & 15) == 0 && dy.ld % 8 == 0 && dy.ld < 1ull << 38; // (a tile map's distances are below 2^40 bytes)
+    const host::Block8GradientPlan plan = host::block8_gradient_plan(a.n_blocks, direct ? groups.twos : 0, x.n, sm_count);
     p.most = plan.most, p.split = plan.split;
     p.groups = groups, p.x = x, p.list = groups.groups[p.most - 1], p.n_groups = groups.count[p.most - 1];
     p.dy = dy.p, p.ld = dy.ld, p.out = out, p.accumulate = accumulate, p.fault = fault;
     p.n_rows = a.n_rows, p.n_cols = a.n_cols;
-    p.stages = kRoom / p.most;
-    p.direct = ((uintptr_t)dy.p & 15) == 0 && dy.ld % 8 == 0 && dy.ld < 1ull << 38; // (a tile map's distances are below 2^40 bytes)
+    p.stages = direct ? kRoom / p.most : kShiftedStages;
+    p.direct = direct;
     CUtensorMap map_dy, map_x;
     cudaError_t e = byte_map(&map_x, x.values, x.ld, x.n, x.ld, kRows, false); // as it lies, without swizzle
     if (e == cudaSuccess && p.direct)
