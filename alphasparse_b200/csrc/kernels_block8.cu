@@ -49,7 +49,7 @@ template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const
 }
 
 // the same the other way
-template <class T> __global__ void __launch_bounds__(256) k_rows8_restore(Rows8Dev x, T *out, uint64_t ld)
+template <class T> __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 6) k_rows8_restore(Rows8Dev x, T *out, uint64_t ld)
 {
     const unsigned lane = threadIdx.x % 32, lane8 = lane % 8, n_blocks = (x.n_cols + 127) / 128, fours = (n_blocks + 3) / 4;
     const unsigned blk = blockIdx.x % fours * 4 + lane / 8, row = blockIdx.x / fours * 8 + threadIdx.x / 32;

@@ -44,8 +44,8 @@ static_assert(kHeld % 2 == 0, "places for x are shared out between two groups of
 constexpr unsigned kUnfolded = 3, kUnfoldedBytes = 2 * kTile; // x in 16 bits: 64 columns after 64 columns, a row t 128 bytes
 constexpr unsigned kThreads = 896;
 // Rows of dy that are not all on 16-byte boundaries cannot be copied by tiles. The warps that unfold x bring them, one of their steps ahead, in the aligned
-// pieces of 16 bytes that they lie in, and shift them to where they belong: twice as long for a step as by tiles (element by element it was
-// 17 times). They then take a part of dy's room, and groups are single blocks.
+// pieces of 16 bytes that they lie in, and shift them to where they belong: 4001 rows, a quarter of 4001 x 4003, take 133 us (450 element by
+// element) where 4096 rows of 4096 x 4096 take 42 by tiles. They then take a part of dy's room, and groups are single blocks.
 constexpr unsigned kPitch = 272, kRawBytes = kRows * kPitch, kShiftedStages = 3; // 17 pieces a row
 static_assert(kShiftedStages * kBlockBytes + 4 * kRawBytes <= kRoom * kBlockBytes, "two steps of each group of warps beside the stages");
 
@@ -276,30 +276,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         // 8 lanes and 16 columns a lane to a row t: 4 rows a warp at once, warp w rows 4 w on, then 32 rows further
         const unsigned lane8 = lane % 8, w = (warp - 12) % 8, row0 = w * 4 + lane / 8, mine = (warp - 12) / 8;
         unsigned s = 0, phase = 0, x = 0, x_phase = 0, h = 0, h_phase = 0, turn = 0, parity = 0;
-        // rows of dy that begin anywhere
-        unsigned char *raws = dys + kShiftedStages * kBlockBytes + mine * 2 * kRawBytes;
-        const auto offset_of = [&](unsigned t, unsigned r0) { return (unsigned)((uintptr_t)p.dy + ((uint64_t)t * p.ld + r0) * 2) & 15u; };
+        // Rows of dy that begin anywhere: a thread has piece j of rows 2 w + lane / 16 + 16 k of a step, which all lie the same number of bytes behind a boundary,
+        // in all steps.
+        const unsigned j = lane % 16, row_dy = 2 * w + lane / 16;
+        unsigned char *raws = dys + kShiftedStages * kBlockBytes + mine * 2 * kRawBytes + row_dy * kPitch + 16 * j;
+        const uintptr_t lo = (uintptr_t)p.dy, hi = lo + ((uint64_t)(p.x.n - 1) * p.ld + p.n_rows) * 2; // dy
+        const unsigned offset = (unsigned)(lo + row_dy * p.ld * 2) & 15u; // (128 r more elements change nothing)
         const auto settle = [&](unsigned &u, unsigned &i) { // step i of the rows, or as much further on in the groups after this one
             while (u < p.n_groups && i >= step1) i -= step1 - step0, u += stride;
         };
         const auto ask = [&](unsigned u, unsigned i, unsigned to) {
             if (u < p.n_groups)
             {
-                const unsigned r0 = p.groups.row[p.groups.from[p.list[u] & 0x7fffffffu]] * 128, j = lane % 16;
-                const uintptr_t lo = (uintptr_t)p.dy, hi = lo + ((uint64_t)(p.x.n - 1) * p.ld + p.n_rows) * 2;
-#pragma unroll
-                for (unsigned k = 0; k < 4; k++)
+                const unsigned r0 = p.groups.row[p.groups.from[p.list[u] & 0x7fffffffu]] * 128;
+                const uintptr_t at = lo + (((uint64_t)i * kRows + row_dy) * p.ld + r0) * 2 - offset + 16 * j, far = 32 * p.ld;
+                unsigned char *piece = raws + to * kRawBytes;
+                if (i > 0 && lo + (((uint64_t)i * kRows + kRows - 1) * p.ld + r0) * 2 + kPitch <= hi) // all of the step's pieces are in dy
                 {
-                    const unsigned row = 16 * k + 2 * w + lane / 16, t = i * kRows + row;
-                    const uintptr_t at = lo + ((uint64_t)t * p.ld + r0) * 2 - offset_of(t, r0) + 16 * j;
-                    uint4 *piece = reinterpret_cast<uint4 *>(raws + to * kRawBytes + row * kPitch) + j;
-                    const auto bring = [&](uint4 *piece, uintptr_t at) {
-                        if (t < p.x.n && at >= lo && at + 16 <= hi) copy16(piece, reinterpret_cast<const void *>(at));
-                        else *piece = t < p.x.n ? load_piece<__half>(at, lo, hi) : make_uint4(0, 0, 0, 0);
-                    };
-                    bring(piece, at);
-                    if (j == 15) bring(piece + 1, at + 16);
+#pragma unroll
+                    for (unsigned k = 0; k < 4; k++)
+                    {
+                        copy16(piece + k * 16 * kPitch, reinterpret_cast<const void *>(at + k * far));
+                        if (j == 15) copy16(piece + k * 16 * kPitch + 16, reinterpret_cast<const void *>(at + k * far + 16));
+                    }
                 }
+                else
+                    for (unsigned k = 0; k < 4; k++)
+                        for (unsigned e = 0; e < (j == 15 ? 2 : 1); e++)
+                            *reinterpret_cast<uint4 *>(piece + k * 16 * kPitch + e * 16) =
+                                i * kRows + row_dy + 16 * k < p.x.n ? load_piece<__half>(at + k * far + e * 16, lo, hi) : make_uint4(0, 0, 0, 0);
             }
             copies_are_one_group();
         };
@@ -356,14 +361,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                         wait_for_all_groups_but<1>();
                         __syncwarp();
                         if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
-                        const unsigned r0 = p.groups.row[p.groups.from[first]] * 128, j = lane % 16;
-                        const int columns = (int)(p.n_rows - r0) - (int)(8 * j); // of the piece, that are in the matrix
+                        const int columns = (int)(p.n_rows - p.groups.row[p.groups.from[first]] * 128) - (int)(8 * j); // of the piece, that are in the matrix
 #pragma unroll
                         for (unsigned k = 0; k < 4; k++)
                         {
-                            const unsigned t = 16 * k + 2 * w + lane / 16, o = offset_of(i * kRows + t, r0);
-                            const uint4 *piece = reinterpret_cast<const uint4 *>(raws + parity * kRawBytes + t * kPitch) + j;
-                            uint4 v = shifted(piece[0], piece[1], o / 4, o % 4 * 8);
+                            const unsigned t = row_dy + 16 * k;
+                            const uint4 *piece = reinterpret_cast<const uint4 *>(raws + parity * kRawBytes + k * 16 * kPitch);
+                            uint4 v = shifted(piece[0], piece[1], offset / 4, offset % 4 * 8);
                             if (columns < 8)
                             {
                                 const auto keep = [&](unsigned word, int e) { return columns > e + 1 ? word : columns > e ? word & 0xffffu : 0u; };

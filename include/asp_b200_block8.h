@@ -18,8 +18,9 @@
  *
  * Sums are in 32 bits and rounded once, when they are stored. All entry points: device pointers aligned to their element type
  * unless said otherwise; ld = distance of two rows in elements, 0 = their length; asynchronous on the context's stream; the context
- * is of the device that the handle was created on. A handle's calls may be captured into a graph, those that create and destroy
- * may not. n == 0 is allowed and touches no row.
+ * is of the device that the handle was created on. A handle's calls may be captured into a graph, which then needs the context and the handles for as
+ * long as it is replayed; those that create and destroy may not. Calls of several contexts are in no order unless the caller gives them one.
+ * n == 0 is allowed and touches no row. Results have the same bits every time.
  */
 #ifndef ASP_B200_BLOCK8_H
 #define ASP_B200_BLOCK8_H
@@ -79,7 +80,8 @@ asp_status asp_block8_product(asp_ctx *ctx, const asp_block8 *m, int transposed,
 /* The gradient of a loss by the stored blocks, from the gradient dY by the rows of y = A x and the rows x kept in 8 bits:
  * dA[block (i, j)] = sum over the rows of dy[128 i + .] x[128 j + .]^T, 32 bits, in the order of asp_block8_set_values; zero outside the
  * matrix. dY: ASP_F16 | ASP_BF16, the type that x was converted from (ASP_ERR_UNSUPPORTED otherwise), so that the products' factors
- * are exact; as many rows as x holds. accumulate != 0: added to d_out. d_out 16-byte aligned. */
+ * are exact; as many rows as x holds. Rows of dY on 16-byte boundaries (d_dy, and ld a multiple of 8) are copied by tiles, others take up to three times as
+ * long. accumulate != 0: added to d_out. d_out 16-byte aligned. Sums of 1280 rows are added up, rounded, in one order. */
 asp_status asp_block8_gradient(asp_ctx *ctx, const asp_block8 *m, const asp_rows8 *x, const void *d_dy, int dtype, uint64_t ld, float *d_out, int accumulate);
 
 #ifdef __cplusplus
