@@ -28,13 +28,12 @@ using namespace block8;
 // where the products take 256. (Four would be 384, but leave no room for a second D: measured the same, with the rows below in one sum.)
 //
 // Tensor cores cut off what they add up to, which over 8192 rows in one sum showed as 6.5e-6 of the result, where sums that are rounded have 6e-7. So D takes
-// 1280 rows (7e-7), then another one the next, while the first is added, rounded, to the sum of those before: in tensor memory where a
-// group is one block, by L2 where it is two (12 % of the time for 8192 rows). A CTA per SM goes through the groups. Where there are few of them a cluster shares the
+// 1280 rows in bf16 (8e-7), 768 in fp16, whose products have more bits (8e-7; 1.4e-6 with 1280), then another one the next, while the first is added,
+// rounded, to the sum of those before: in tensor memory where a group is one block, by L2 where it is two (12 % of the time for 8192 rows). A CTA per SM goes through the groups. Where there are few of them a cluster shares the
 // rows of one; its CTAs then add to the result one after the other, each beginning with another part of it: the same order, and bits, every time.
 //
 // Warp 0 copies, warp 1 issues products, warps 4 to 11 add up and store, warps 12 to 19 and 20 to 27 unfold x, every second step each.
 constexpr unsigned kRows = host::kBlock8GradientRows; // t a step
-constexpr unsigned kRound = 1280 / kRows;             // steps a sum
 constexpr unsigned kTile = kRows * 128; // bytes of 64 columns of a step's rows in 16 bits, of 128 in 8
 constexpr unsigned kRoom = 8, kBlockBytes = 2 * kTile;        // dy: blocks of a step's rows, as many steps as fit
 constexpr unsigned kHeld = 4, kHeldBytes = kTile + 1024;      // x in 8 bits, and its scales
@@ -76,6 +75,7 @@ struct Shared
 struct Unfold16 // to fp16: in two factors, since the power may be below what fp16 has (the product is not, as x was fp16)
 {
     static constexpr bool bf16 = false;
+    static constexpr unsigned round = 768 / kRows; // steps a sum
     static __device__ __forceinline__ void words(uint4 q, unsigned scale, unsigned *out)
     {
         const int k1 = max((int)scale, 127 - 14);
@@ -96,6 +96,7 @@ struct Unfold16 // to fp16: in two factors, since the power may be below what fp
 struct UnfoldB16
 {
     static constexpr bool bf16 = true;
+    static constexpr unsigned round = 1280 / kRows;
     static __device__ __forceinline__ void words(uint4 q, unsigned scale, unsigned *out)
     {
         const unsigned in[4] = {q.x, q.y, q.z, q.w};
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                     if (fresh)
                     {
                         if (!tc::barrier_wait(&sh.taken[d], d_phase ^ 1, &sh.gave_up)) goto end;
-                        left = kRound;
+                        left = Unfold::round;
                     }
                     if (p.direct && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
                     if (!tc::barrier_wait(&sh.unfolded[h], h_phase, &sh.gave_up)) goto end;
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         }
         for (unsigned u = u0; u < p.n_groups; u += stride)
         {
-            const unsigned first = p.list[u] & 0x7fffffffu, blocks = 1 + (p.list[u] >> 31), byte = p.groups.col[p.groups.from[first]] % 4;
+            const unsigned first = p.list[u] & 0x7fffffffu, byte = p.groups.col[p.groups.from[first]] % 4;
             for (unsigned i = step0; i < step1; i++)
             {
                 if (turn == mine)
@@ -326,11 +327,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                     uint4 q[2];
                     unsigned scale[2];
 #pragma unroll
-                    for (unsigned j = 0; j < 2; j++)
+                    for (unsigned n = 0; n < 2; n++)
                     {
-                        const unsigned t = row0 + 32 * j, row = i * kRows + t;
-                        q[j] = *reinterpret_cast<const uint4 *>(from + t * 128 + 16 * lane8);
-                        scale[j] = row < p.x.n ? from[kTile + row0 * 16 + row / 32 % 4 * 4 + byte] : 127; // (rows behind the last one are zeros, with any scale)
+                        const unsigned t = row0 + 32 * n, row = i * kRows + t;
+                        q[n] = *reinterpret_cast<const uint4 *>(from + t * 128 + 16 * lane8);
+                        scale[n] = row < p.x.n ? from[kTile + row0 * 16 + row / 32 % 4 * 4 + byte] : 127; // (rows behind the last one are zeros, with any scale)
                     }
                     // The next copy may come while these are unfolded. Reads and copies are of different proxies: without the fence a copy overtook reads that
                     // other kernels' warps held up.
@@ -340,11 +341,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                     if (!tc::barrier_wait(&sh.used[h], h_phase ^ 1, &sh.gave_up)) goto end;
                     unsigned char *to = halves + h * kUnfoldedBytes + lane8 / 4 * kTile;
 #pragma unroll
-                    for (unsigned j = 0; j < 2; j++)
+                    for (unsigned n = 0; n < 2; n++)
                     {
-                        const unsigned t = row0 + 32 * j;
+                        const unsigned t = row0 + 32 * n;
                         unsigned v[8];
-                        Unfold::words(q[j], scale[j], v);
+                        Unfold::words(q[n], scale[n], v);
                         // 16-byte pieces 2 l and 2 l + 1 of the row's 128 bytes, swapped in the second half so that eight lanes meet no conflict
                         unsigned char *line = to + t * 128;
                         const unsigned at = lane8 % 4 * 2, second = lane8 / 4;
@@ -397,11 +398,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         {
             const unsigned blocks = 1 + (p.list[u] >> 31);
             const Places at = places<Unfold>(p, p.list[u], quarter, lane);
-            for (unsigned i = step0; i < step1; i += kRound)
+            for (unsigned i = step0; i < step1; i += Unfold::round)
             {
                 if (!tc::barrier_wait<64>(&sh.done[d], d_phase, &sh.gave_up)) goto end;
                 tc::fence_after();
-                const bool last = i + kRound >= step1 && p.split == 1;
+                const bool last = i + Unfold::round >= step1 && p.split == 1;
                 for (unsigned c = mine; c < blocks * 128; c += 32)
                 {
                     float v[16];
