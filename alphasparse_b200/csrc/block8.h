@@ -12,9 +12,8 @@ struct Block8Dev
     const uint8_t *values;  // [blocks][128][128], row by row
     const uint8_t *scales;  // [blocks]: exponent + 127
     const uint8_t *scale_rows; // [blocks][512]: the same byte, once for each row of the block and each word, as tensor memory takes it
-    const unsigned *ptr;    // [block rows + 1]
     const unsigned *col;    // [blocks]
-    const unsigned *order;  // block rows, longest first
+    const uint4 *rows;      // block rows, longest first: {which one, its first block, number of its blocks, 0}
     unsigned n_block_rows, n_blocks, longest;
     unsigned n_rows, n_cols; // of the matrix: lengths of a row of Y and of X
 };

@@ -95,15 +95,16 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
         return r;
     };
     const int sides = m->transposed ? 2 : 1;
-    Piece values[2], scales[2], scale_rows[2], ptr[2], col[2], order[2];
+    Piece values[2], scales[2], scale_rows[2], col[2], rows_of[2];
+    std::vector<uint4> by_length[2];
     for (int s = 0; s < sides; s++)
     {
         values[s] = take(n * kBlock8 * kBlock8);
         scales[s] = take(n);
         scale_rows[s] = take(n * 512);
-        ptr[s] = take(p.side[s].ptr.size() * 4);
         col[s] = take(n * 4);
-        order[s] = take(p.side[s].order.size() * 4);
+        for (const uint32_t r : p.side[s].order) by_length[s].push_back({r, p.side[s].ptr[r], p.side[s].ptr[r + 1] - p.side[s].ptr[r], 0});
+        rows_of[s] = take(by_length[s].size() * sizeof(uint4));
     }
     const Piece row = take(n * 4), place = take(n * 4), from = take(n * 4);
     Piece groups[2];
@@ -132,9 +133,8 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
         d.values = m->set[s].values = base + values[s].at;
         d.scales = m->set[s].scales = base + scales[s].at;
         d.scale_rows = m->set[s].scale_rows = base + scale_rows[s].at;
-        d.ptr = send(ptr[s], h.ptr.data());
         d.col = send(col[s], h.col.data());
-        d.order = send(order[s], h.order.data());
+        d.rows = reinterpret_cast<const uint4 *>(send(rows_of[s], by_length[s].data()));
         d.n_block_rows = h.rows(), d.n_blocks = (unsigned)n, d.longest = h.longest;
         d.n_rows = (unsigned)(s ? p.n_cols : p.n_rows), d.n_cols = (unsigned)(s ? p.n_rows : p.n_cols);
         e = cudaMemsetAsync(base + values[s].at, 0, values[s].bytes, ctx->stream);

@@ -31,12 +31,18 @@ using namespace block8;
 // Where there are fewer tiles than SMs, a cluster shares the blocks of a tile; its CTAs put their sums into shared memory and add them up in order,
 // some columns each.
 //
+// What bounds it is shared memory, 128 bytes a clock and SM: a step writes 40 KB to it and the products read 40 KB, 640 clocks where the products alone
+// take 384. Rows, columns and rows of X, share of blocks stored: 8192, 8192, 8192, half: 247 us, 2.23 PFLOP/s in a burst; called over and over the chip comes to its
+// power limit and 1.28 GHz, and it takes 303. 4096, 4096, 2048, a quarter: 18 us, 0.95 PFLOP/s (512 tiles over 148 SMs, the last wave half empty,
+// and each CTA's first copies and last stores).
+//
 // A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 9 store.
 constexpr unsigned kMostRows = host::kBlock8ProductRows;
 constexpr unsigned kStages = 8; // at most
 constexpr unsigned kScaleBytes = 512 + 1024;
 constexpr unsigned kRoom = 221 * 1024; // of shared memory for stages
 constexpr unsigned kThreads = 320;
+constexpr uint64_t kNear = 40ull << 20;
 
 struct ProductArgs
 {
@@ -45,7 +51,7 @@ struct ProductArgs
     void *y;
     uint64_t ldy;
     unsigned tile;   // rows of X a tile, a multiple of 64
-    unsigned tiles_x, group;
+    unsigned tiles_x, wide;
     unsigned n_tiles;
     unsigned split;  // CTAs that share a tile's blocks; then a CTA has one tile
     unsigned stages, stage_bytes;
@@ -59,27 +65,42 @@ struct Shared
     unsigned tensor, gave_up;
 };
 
-// The steps of a CTA, in order: the blocks of its tiles. A tile is given by its place among tiles in groups of `group` block rows times all tiles of X, so
-// that the tiles that run at the same time share blocks of A and rows of X in L2.
+// The steps of a CTA, in order: the blocks of its tiles. Tiles are in the order of their block rows, longest first, and handed out to the CTAs forwards and backwards in
+// turn, so that who has a long one gets a short one next (a quarter of 4096 x 4096 by 2048 rows: SCHED_A us, SCHED_B with block rows side by side and always forwards).
+// Where X is larger than a part of L2 it is gone through in parts of `wide` tiles, each with all block rows.
 struct Steps
 {
     const ProductArgs &p;
-    unsigned tile, j = 0, end = 0, row = 0, t0 = 0;
-    __device__ __forceinline__ explicit Steps(const ProductArgs &args) : p(args), tile(blockIdx.x / args.split) { locate(); }
-    __device__ __forceinline__ bool valid() const { return tile < p.n_tiles; }
-    __device__ __forceinline__ void locate()
+    bool valid;
+    unsigned j, end, row, t0;
+    __device__ __forceinline__ explicit Steps(const ProductArgs &args) : p(args), tile(blockIdx.x / args.split)
     {
-        if (!valid()) return;
-        const unsigned per = p.group * p.tiles_x, g = tile / per, in = tile % per, rows = min(p.group, p.a.n_block_rows - g * p.group);
-        row = p.a.order[g * p.group + in % rows];
-        t0 = in / rows * p.tile;
-        const unsigned lo = p.a.ptr[row], len = p.a.ptr[row + 1] - lo, piece = blockIdx.x % p.split;
-        j = lo + len * piece / p.split, end = lo + len * (piece + 1) / p.split; // (less than 2^24 blocks, 8 pieces at most)
+        ask();
+        next_tile();
     }
     __device__ __forceinline__ void next_tile()
     {
-        tile += gridDim.x / p.split;
-        locate();
+        valid = tile < p.n_tiles;
+        if (!valid) return;
+        row = next.x, t0 = next_t0;
+        const unsigned piece = blockIdx.x % p.split;
+        j = next.y + next.z * piece / p.split, end = next.y + next.z * (piece + 1) / p.split; // (less than 2^24 blocks, 8 pieces at most)
+        turn++;
+        if (turn > p.n_tiles / gridDim.x || p.split > 1) tile = p.n_tiles; // (a cluster has one tile only)
+        else tile = turn * gridDim.x + (turn % 2 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        ask();
+    }
+
+  private:
+    unsigned tile, turn = 0; // of the tile after this one, whose block row is on its way
+    uint4 next;
+    unsigned next_t0;
+    __device__ __forceinline__ void ask()
+    {
+        if (tile >= p.n_tiles) return;
+        const unsigned per = p.wide * p.a.n_block_rows, part = tile / per, in = tile % per, columns = min(p.wide, p.tiles_x - part * p.wide);
+        next = p.a.rows[in / columns];
+        next_t0 = (part * p.wide + in % columns) * p.tile;
     }
 };
 
@@ -148,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
     __syncthreads();
     tc::fence_after();
     const unsigned tensor = sh.tensor;
+    Steps at(p);
     grid_wait();
     grid_release();
     const unsigned x_bytes = p.tile * 128;
@@ -157,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
         if (tc::one_lane())
         {
             unsigned s = 0, phase = 0;
-            for (Steps at(p); at.valid(); at.next_tile())
+            for (; at.valid; at.next_tile())
                 for (; at.j < at.end; at.j++)
                 {
                     const unsigned col = p.a.col[at.j];
@@ -182,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
             // have no more than two or three products waiting.
             unsigned s = 0, phase = 0, b = 0, b_phase = 0, turn = 0;
             bool ready = false;
-            for (Steps at(p); at.valid(); at.next_tile())
+            for (; at.valid; at.next_tile())
             {
                 if (at.j == at.end) continue;
                 if (!tc::barrier_wait(&sh.taken[b], b_phase ^ 1, &sh.gave_up)) goto end;
@@ -224,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
     {
         unsigned b = 0, b_phase = 0;
         const unsigned quarter = warp % 4, first = (warp - 2) / 4 * 32; // two warps to a quarter of D's lanes, every second 32 columns each
-        for (Steps at(p); at.valid(); at.next_tile())
+        for (; at.valid; at.next_tile())
         {
             const unsigned row0 = at.row * 128 + quarter * 32, limit = min(p.x.n, at.t0 + p.tile);
             float v[32];
@@ -272,7 +294,7 @@ end:
         const cg::cluster_group cluster = cg::this_cluster();
         const float *part = reinterpret_cast<const float *>(stages);
         cluster.sync();
-        const Steps at(p);
+        const Steps at(p); // (those that copy and multiply have gone on)
         Y *y = reinterpret_cast<Y *>(p.y);
         const unsigned rows = min(128u, p.a.n_rows - at.row * 128), columns = min(p.tile, p.x.n - at.t0);
         for (unsigned i = threadIdx.x + kThreads * (blockIdx.x % p.split); i < columns * 32; i += kThreads * p.split)
@@ -334,9 +356,15 @@ cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const D
     const uint64_t tiles = (uint64_t)a.n_block_rows * p.tiles_x;
     if (tiles > 0xf0000000u) return cudaErrorInvalidValue; // (2^38 rows of blocks' results and more)
     p.n_tiles = (unsigned)tiles;
-    // block rows that run together: as many bytes of A as of X
-    const double side = (double)p.tile * x.ld / std::max(1.0, 16384.0 * a.n_blocks / a.n_block_rows);
-    p.group = std::min<unsigned>(a.n_block_rows, std::max(1u, (unsigned)sqrt(sm_count * side)));
+    // Tiles of X that are gone through together: all where X stays in L2 at hand (8192 x 8192 bytes do not), else so many that the tiles that run at the same time
+    // have as many bytes of A as of X.
+    p.wide = p.tiles_x;
+    if (x.n * x.ld > kNear)
+    {
+        const double side = 16384.0 * a.n_blocks / a.n_block_rows / (p.tile * x.ld);
+        const unsigned parts = (p.tiles_x + std::max(1u, (unsigned)(sqrt(sm_count * side) + 0.5)) - 1) / std::max(1u, (unsigned)(sqrt(sm_count * side) + 0.5));
+        p.wide = (p.tiles_x + parts - 1) / parts;
+    }
     p.stage_bytes = (16384 + p.tile * 128 + kScaleBytes + 1023) / 1024 * 1024;
     p.stages = std::min(kStages, kRoom / p.stage_bytes);
     p.pairs = y.dtype != ASP_F32 && ((uintptr_t)y.p & 3) == 0 && y.ld % 2 == 0;
