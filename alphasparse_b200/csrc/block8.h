@@ -59,12 +59,14 @@ cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st);
 cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, cudaStream_t st);
 // many rows in 8 bits. fault: a word that the kernel sets when it gives up a wait
 cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st);
-// The blocks by block column, in groups (Block8Pattern)
+// The blocks by block column, in groups (Block8Pattern): everything about a group in one place, since each look-up waits for the one before
+struct alignas(16) Block8Group
+{
+    unsigned block[2], row[2], col, n; // blocks of A, their block rows, their block column, how many
+};
 struct Block8Groups
 {
-    const unsigned *row, *col;   // of each block of A
-    const unsigned *from;        // block of A^T -> block of A
-    const unsigned *groups[2];
+    const Block8Group *groups[2];
     unsigned count[2], twos;
 };
 cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &groups, const Rows8Dev &x, const Dense &dy, float *out, bool accumulate, int sm_count, unsigned *fault, cudaStream_t st);

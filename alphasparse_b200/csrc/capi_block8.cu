@@ -106,11 +106,23 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
         for (const uint32_t r : p.side[s].order) by_length[s].push_back({r, p.side[s].ptr[r], p.side[s].ptr[r + 1] - p.side[s].ptr[r], 0});
         rows_of[s] = take(by_length[s].size() * sizeof(uint4));
     }
-    const Piece row = take(n * 4), place = take(n * 4), from = take(n * 4);
-    Piece groups[2];
-    for (int g = 0; g < 2; g++) groups[g] = take(p.groups[g].size() * 4);
+    const Piece row = take(n * 4), place = take(n * 4);
     std::vector<uint32_t> rows(n);
     for (uint32_t r = 0; r < p.side[0].rows(); r++) std::fill(rows.begin() + p.side[0].ptr[r], rows.begin() + p.side[0].ptr[r + 1], r);
+    Piece groups[2];
+    std::vector<asp::Block8Group> group[2];
+    for (int g = 0; g < 2; g++)
+    {
+        for (const uint32_t u : p.groups[g])
+        {
+            asp::Block8Group of = {};
+            of.n = 1 + (u >> 31);
+            for (uint32_t k = 0; k < of.n; k++) of.block[k] = p.from[(u & 0x7fffffffu) + k], of.row[k] = rows[of.block[k]];
+            of.col = p.side[0].col[of.block[0]];
+            group[g].push_back(of);
+        }
+        groups[g] = take(group[g].size() * sizeof(asp::Block8Group));
+    }
     ASP_ON_DEVICE(ctx);
     m->room.device = ctx->device;
     cudaError_t e = asp::device_alloc(ctx->device, at, &m->room.base, &m->room.got);
@@ -144,11 +156,9 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
     }
     m->row = send(row, rows.data());
     m->place = send(place, p.place.data());
-    m->groups.row = m->row, m->groups.col = m->side[0].col;
-    m->groups.from = send(from, p.from.data());
     for (int g = 0; g < 2; g++)
     {
-        m->groups.groups[g] = send(groups[g], p.groups[g].data());
+        m->groups.groups[g] = reinterpret_cast<const asp::Block8Group *>(send(groups[g], group[g].data()));
         m->groups.count[g] = (unsigned)p.groups[g].size();
     }
     m->groups.twos = p.twos;

@@ -52,9 +52,8 @@ static_assert(kShiftedStages * kBlockBytes + 4 * kRawBytes <= kRoom * kBlockByte
 
 struct GradientArgs
 {
-    Block8Groups groups;
     Rows8Dev x;
-    const unsigned *list; // groups of blocks
+    const Block8Group *list;
     unsigned n_groups, most;
     const void *dy;
     uint64_t ld;
@@ -130,23 +129,22 @@ struct UnfoldB16
 // the column of a block that D's lane has
 template <class Unfold> __device__ __forceinline__ unsigned column_of(unsigned lane) { return Unfold::bf16 && (lane % 4 == 1 || lane % 4 == 2) ? lane ^ 3 : lane; }
 
-// Where a lane's part of a group's blocks goes: looked up once a group, as each look-up waits for the one before
+// Where a lane's part of a group's blocks goes
 struct Places
 {
     float *to[2];     // element (0, c) of each block
     unsigned rows[2]; // of them inside the matrix; 0: the column is not
 };
-template <class Unfold> __device__ __forceinline__ Places places(const GradientArgs &p, unsigned group, unsigned quarter, unsigned lane)
+template <class Unfold> __device__ __forceinline__ Places places(const GradientArgs &p, const Block8Group &group, unsigned quarter, unsigned lane)
 {
-    const unsigned first = group & 0x7fffffffu, c = quarter * 32 + column_of<Unfold>(lane);
+    const unsigned c = quarter * 32 + column_of<Unfold>(lane);
     Places at = {};
 #pragma unroll
     for (unsigned k = 0; k < 2; k++)
-        if (k == 0 || group >> 31)
+        if (k < group.n)
         {
-            const unsigned b = p.groups.from[first + k];
-            at.to[k] = p.out + (uint64_t)b * 16384 + c;
-            at.rows[k] = p.groups.col[b] * 128 + c < p.n_cols ? min(128u, p.n_rows - p.groups.row[b] * 128) : 0;
+            at.to[k] = p.out + (uint64_t)group.block[k] * 16384 + c;
+            at.rows[k] = group.col * 128 + c < p.n_cols ? min(128u, p.n_rows - group.row[k] * 128) : 0;
         }
     return at;
 }
@@ -199,6 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
     __syncthreads();
     tc::fence_after();
     const unsigned tensor = sh.tensor;
+    const Block8Group first = p.list[u0];
     grid_wait();
     grid_release();
 
@@ -209,8 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
             unsigned s = 0, phase = 0, x = 0, x_phase = 0;
             for (unsigned u = u0; u < p.n_groups; u += stride)
             {
-                const unsigned first = p.list[u] & 0x7fffffffu, blocks = 1 + (p.list[u] >> 31), col = p.groups.col[p.groups.from[first]];
-                const unsigned r[2] = {p.groups.row[p.groups.from[first]] * 128, blocks > 1 ? p.groups.row[p.groups.from[first + 1]] * 128 : 0};
+                const Block8Group group = u == u0 ? first : p.list[u];
+                const unsigned blocks = group.n, col = group.col;
                 for (unsigned i = step0; i < step1; i++)
                 {
                     const int t = (int)(i * kRows);
@@ -228,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                     for (unsigned k = 0; k < 2; k++)
                         if (k < blocks)
                         {
-                            tc::copy_tile(to + k * kBlockBytes, &map_dy, (int)r[k], t, &sh.full[s]);
-                            tc::copy_tile(to + k * kBlockBytes + kTile, &map_dy, (int)r[k] + 64, t, &sh.full[s]);
+                            tc::copy_tile(to + k * kBlockBytes, &map_dy, (int)group.row[k] * 128, t, &sh.full[s]);
+                            tc::copy_tile(to + k * kBlockBytes + kTile, &map_dy, (int)group.row[k] * 128 + 64, t, &sh.full[s]);
                         }
                     if (++s == p.stages) s = 0, phase ^= 1;
                 }
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
             unsigned s = 0, phase = 0, h = 0, h_phase = 0, d = 0, d_phase = 0;
             for (unsigned u = u0; u < p.n_groups; u += stride)
             {
-                const unsigned shape = tc::halves(128 + 128 * (p.list[u] >> 31), Unfold::bf16);
+                const unsigned shape = tc::halves(128 * (u == u0 ? first.n : p.list[u].n), Unfold::bf16);
                 for (unsigned i = step0, left = 0; i < step1; i++)
                 {
                     const bool fresh = left == 0;
@@ -291,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         const auto ask = [&](unsigned u, unsigned i, unsigned to) {
             if (u < p.n_groups)
             {
-                const unsigned r0 = p.groups.row[p.groups.from[p.list[u] & 0x7fffffffu]] * 128;
+                const unsigned r0 = p.list[u].row[0] * 128;
                 const uintptr_t at = lo + (((uint64_t)i * kRows + row_dy) * p.ld + r0) * 2 - offset + 16 * j, far = 32 * p.ld;
                 unsigned char *piece = raws + to * kRawBytes;
                 if (i > 0 && lo + (((uint64_t)i * kRows + kRows - 1) * p.ld + r0) * 2 + kPitch <= hi) // all of the step's pieces are in dy
@@ -319,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         }
         for (unsigned u = u0; u < p.n_groups; u += stride)
         {
-            const unsigned first = p.list[u] & 0x7fffffffu, byte = p.groups.col[p.groups.from[first]] % 4;
+            const unsigned byte = (u == u0 ? first.col : p.list[u].col) % 4, row = u == u0 ? first.row[0] : p.list[u].row[0];
             for (unsigned i = step0; i < step1; i++)
             {
                 if (turn == mine)
@@ -331,9 +330,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
 #pragma unroll
                     for (unsigned n = 0; n < 2; n++)
                     {
-                        const unsigned t = row0 + 32 * n, row = i * kRows + t;
+                        const unsigned t = row0 + 32 * n, at = i * kRows + t;
                         q[n] = *reinterpret_cast<const uint4 *>(from + t * 128 + 16 * lane8);
-                        scale[n] = row < p.x.n ? from[kTile + row0 * 16 + row / 32 % 4 * 4 + byte] : 127; // (rows behind the last one are zeros, with any scale)
+                        scale[n] = at < p.x.n ? from[kTile + row0 * 16 + at / 32 % 4 * 4 + byte] : 127; // (rows behind the last one are zeros, with any scale)
                     }
                     // The next copy may come while these are unfolded. Reads and copies are of different proxies: without the fence a copy overtook reads that
                     // other kernels' warps held up.
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                         wait_for_all_groups_but<1>();
                         __syncwarp();
                         if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
-                        const int columns = (int)(p.n_rows - p.groups.row[p.groups.from[first]] * 128) - (int)(8 * j); // of the piece, that are in the matrix
+                        const int columns = (int)(p.n_rows - row * 128) - (int)(8 * j); // of the piece, that are in the matrix
 #pragma unroll
                         for (unsigned k = 0; k < 4; k++)
                         {
@@ -398,8 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
         const unsigned quarter = warp % 4, mine = (warp - 4) / 4 * 16;
         for (unsigned u = u0; u < p.n_groups; u += stride)
         {
-            const unsigned blocks = 1 + (p.list[u] >> 31);
-            const Places at = places<Unfold>(p, p.list[u], quarter, lane);
+            const Block8Group group = u == u0 ? first : p.list[u];
+            const unsigned blocks = group.n;
+            const Places at = places<Unfold>(p, group, quarter, lane);
             for (unsigned i = step0; i < step1; i += Unfold::round)
             {
                 if (!tc::barrier_wait<64>(&sh.done[d], d_phase, &sh.gave_up)) goto end;
@@ -441,7 +441,7 @@ end:
     // together, whatever became of their waits.)
     if (p.split > 1)
     {
-        const Places at = places<Unfold>(p, p.list[u0], warp % 4, lane);
+        const Places at = places<Unfold>(p, first, warp % 4, lane);
         const unsigned width = 128 / p.split;
         for (unsigned turn = 0; turn < p.split; turn++)
         {
@@ -488,7 +488,7 @@ cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &group
     const bool direct = ((uintptr_t)dy.p & 15) == 0 && dy.ld % 8 == 0 && dy.ld < 1ull << 38; // (a tile map's distances are below 2^40 bytes)
     const host::Block8GradientPlan plan = host::block8_gradient_plan(a.n_blocks, direct ? groups.twos : 0, x.n, sm_count);
     p.most = plan.most, p.split = plan.split;
-    p.groups = groups, p.x = x, p.list = groups.groups[p.most - 1], p.n_groups = groups.count[p.most - 1];
+    p.x = x, p.list = groups.groups[p.most - 1], p.n_groups = groups.count[p.most - 1];
     p.dy = dy.p, p.ld = dy.ld, p.out = out, p.accumulate = accumulate, p.fault = fault;
     p.n_rows = a.n_rows, p.n_cols = a.n_cols;
     p.stages = direct ? kRoom / p.most : kShiftedStages;
