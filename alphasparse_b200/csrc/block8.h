@@ -55,9 +55,10 @@ struct Block8Set
 // blocks [first, end) (from: the values of block `first` on); row: block row of each block; place: where it lies among the blocks of A^T
 cudaError_t launch_block8_set(const Block8Dev &a, const unsigned *row, const unsigned *place, const Block8Set to[2], const void *from, int dtype, unsigned first, unsigned end, cudaStream_t st);
 cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st);
-// a few rows: X as it is (held == NULL) or in 8 bits
-cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, cudaStream_t st);
-// many rows in 8 bits. fault: a word that the kernel sets when it gives up a wait
+// a few rows, up to 32: X as it is (held == NULL) or in 8 bits. fault: a word that a kernel sets when it gives up a wait
+cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st);
+cudaError_t launch_block8_batch(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st);
+// many rows in 8 bits
 cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st);
 // The blocks by block column, in groups (Block8Pattern): everything about a group in one place, since each look-up waits for the one before
 struct alignas(16) Block8Group

@@ -6,6 +6,8 @@
 #include <stdint.h>
 #include <string.h>
 
+#include "block8.h"
+
 namespace asp
 {
 namespace block8
@@ -127,10 +129,9 @@ template <class T> struct Raw
         for (int i = 0; i < pieces; i++) w[i] = load_piece<T>(at + 128 * i, (uintptr_t)lo, (uintptr_t)hi);
         if (o && lane8 == 7) more = load_piece<T>(at + 128 * (pieces - 1) + 16, (uintptr_t)lo, (uintptr_t)hi);
     }
-    // all lanes of the warp take part; `columns` of the block are in the row, zeros behind them
-    __device__ __forceinline__ void floats(float *v, unsigned lane8, unsigned columns) const
+    // the lane's elements; all lanes of the warp take part; `columns` of the block are in the row, zeros behind them
+    __device__ __forceinline__ void elements(uint4 *u, unsigned lane8, unsigned columns) const
     {
-        uint4 u[pieces];
         const unsigned lane = threadIdx.x % 32, beside = lane8 < 7 ? lane + 1 : lane - 7;
         if (__any_sync(~0u, words | bits))
         {
@@ -146,14 +147,15 @@ template <class T> struct Raw
         else
 #pragma unroll
             for (int i = 0; i < pieces; i++) u[i] = w[i];
-        T e[16];
-        memcpy(e, u, sizeof(u));
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = to_float(e[i]);
         if (columns < 128)
+        {
+            T e[16];
+            memcpy(e, u, sizeof(e));
 #pragma unroll
             for (int i = 0; i < 16; i++)
-                if (column_in_block<T>(i, lane8) >= columns) v[i] = 0.f;
+                if (column_in_block<T>(i, lane8) >= columns) e[i] = from_float<T>(0.f);
+            memcpy(u, e, sizeof(e));
+        }
     }
 };
 // The scale of what the eight lanes of a block have, and whether something infinite is among it. All lanes of the warp take part. (fmaxf passes NaN over;
@@ -183,6 +185,117 @@ __device__ __forceinline__ void pack16(const float *v, unsigned scale, bool infi
 #pragma unroll
     for (int i = 0; i < 4; i++) q[i] = infinite ? pack4<true>(v + 4 * i, inv) : pack4<false>(v + 4 * i, inv);
 }
+template <class T> __device__ __forceinline__ unsigned floats_to_eight(const uint4 *u, unsigned *q)
+{
+    T e[16];
+    memcpy(e, u, sizeof(e));
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = to_float(e[i]);
+    bool infinite;
+    const unsigned scale = scale_of_8(v, infinite);
+    pack16(v, scale, infinite, q);
+    return scale;
+}
+// Both at once: what the eight lanes of a block have (Raw::elements) to 8 bits, and the scale. All lanes of the warp take part.
+template <class T> __device__ __forceinline__ unsigned to_eight(const uint4 *u, unsigned *q) { return floats_to_eight<T>(u, q); }
+// 16-bit types two elements at a time: the largest, and the division, which is exact, or leaves something that is zero in 8 bits. What is infinite,
+// and numbers near fp16's smallest, whose scales it does not have, go by 32 bits.
+template <class Two> __device__ __forceinline__ float largest_of_8(const Two *e)
+{
+    Two most = __habs2(e[0]); // (the larger of a number and NaN is the number)
+#pragma unroll
+    for (int i = 1; i < 8; i++) most = __hmax2(most, __habs2(e[i]));
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) most = __hmax2(most, __shfl_xor_sync(~0u, most, d));
+    return fmaxf(fmaxf(to_float(most.x), to_float(most.y)), 0.f);
+}
+template <> __device__ __forceinline__ unsigned to_eight<__nv_bfloat16>(const uint4 *u, unsigned *q)
+{
+    __nv_bfloat162 e[8];
+    memcpy(e, u, sizeof(e));
+    const float most = largest_of_8(e);
+    if (__any_sync(~0u, isinf(most))) return floats_to_eight<__nv_bfloat16>(u, q);
+    const unsigned scale = scale_of(most);
+    const __nv_bfloat162 inv = __float2bfloat162_rn(inverse(scale));
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+    {
+        const float2 v = __bfloat1622float2(__hmul2(e[i], inv));
+        unsigned short two;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v.y), "f"(v.x));
+        q[i / 2] = i % 2 ? q[i / 2] | (unsigned)two << 16 : two;
+    }
+    return scale;
+}
+template <> __device__ __forceinline__ unsigned to_eight<__half>(const uint4 *u, unsigned *q)
+{
+    __half2 e[8];
+    memcpy(e, u, sizeof(e));
+    const float most = largest_of_8(e);
+    if (__any_sync(~0u, isinf(most) || (most > 0.f && most < 0x1p-21f))) return floats_to_eight<__half>(u, q);
+    const unsigned scale = scale_of(most);
+    const int up = most > 0.f ? 127 - (int)scale : 0, first = min(up, 15); // -8 to 30
+    const __half2 f1 = __float2half2_rn(power((unsigned)(127 + first))), f2 = __float2half2_rn(power((unsigned)(127 + up - first)));
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+    {
+        const __half2 v = __hmul2(__hmul2(e[i], f1), f2);
+        unsigned short two;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(two) : "r"(*reinterpret_cast<const unsigned *>(&v)));
+        q[i / 2] = i % 2 ? q[i / 2] | (unsigned)two << 16 : two;
+    }
+    return scale;
+}
+// Rows X of a product: as the caller has them (of type X), or in 8 bits already (Held)
+struct Held
+{
+};
+struct XRows
+{
+    const void *p;
+    uint64_t ld;
+    unsigned n, n_cols;
+    Rows8Dev held;
+};
+// What lane `lane8` of 8 has of a row's block on its way
+template <class X> struct Fetched
+{
+    Raw<X> raw;
+    unsigned columns; // of the block that are in the row
+    __device__ __forceinline__ void ask(const XRows &rows, unsigned row, unsigned kb, unsigned lane8)
+    {
+        const X *x = reinterpret_cast<const X *>(rows.p);
+        columns = rows.n_cols - kb * 128;
+        raw.load(x + row * rows.ld + kb * 128, x, x + (rows.n - 1) * rows.ld + rows.n_cols, lane8);
+    }
+    // 16 elements in 8 bits, element i that of column column(i, lane8), and their scale. All lanes of the warp take part.
+    __device__ __forceinline__ unsigned eight(unsigned *q, unsigned lane8) const
+    {
+        uint4 u[Raw<X>::pieces];
+        raw.elements(u, lane8, columns);
+        return to_eight<X>(u, q);
+    }
+    static constexpr int per = 16 / sizeof(X); // elements side by side
+    static __device__ __forceinline__ unsigned column(int i, unsigned lane8) { return column_in_block<X>(i, lane8); }
+};
+template <> struct Fetched<Held>
+{
+    uint4 v;
+    unsigned scale;
+    __device__ __forceinline__ void ask(const XRows &rows, unsigned row, unsigned kb, unsigned lane8)
+    {
+        v = *reinterpret_cast<const uint4 *>(rows.held.values + row * rows.held.ld + kb * 128 + 16 * lane8);
+        scale = rows.held.scales[scale_at(rows.held, row, kb)];
+    }
+    __device__ __forceinline__ unsigned eight(unsigned *q, unsigned) const
+    {
+        q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w;
+        return scale;
+    }
+    static constexpr int per = 16;
+    static __device__ __forceinline__ unsigned column(int i, unsigned lane8) { return 16 * lane8 + i; }
+};
 // and to where they belong; `to` is the block's first byte
 template <class T> __device__ __forceinline__ void store_block(const unsigned *q, unsigned lane8, uint8_t *to)
 {

@@ -355,7 +355,7 @@ asp_status asp_block8_apply(asp_ctx *ctx, const asp_block8 *m, int transposed, c
     ASP_TRY(look_at(d_y, y_dtype, n, a->n_rows, ldy, "y", &y));
     ASP_TRY(same_device(ctx, m->room));
     ASP_ON_DEVICE(ctx);
-    return launched(asp::launch_block8_few(*a, &x, nullptr, (unsigned)n, y, ctx->sm_count, ctx->stream));
+    return launched(asp::launch_block8_few(*a, &x, nullptr, (unsigned)n, y, ctx->sm_count, ctx->fault, ctx->stream));
 }
 
 asp_status asp_block8_product(asp_ctx *ctx, const asp_block8 *m, int transposed, const asp_rows8 *x, void *d_y, int y_dtype, uint64_t ldy)
@@ -369,7 +369,7 @@ asp_status asp_block8_product(asp_ctx *ctx, const asp_block8 *m, int transposed,
     ASP_TRY(same_device(ctx, m->room));
     ASP_TRY(same_device(ctx, x->room));
     ASP_ON_DEVICE(ctx);
-    if (x->dev.n <= ASP_BLOCK8_APPLY_ROWS) return launched(asp::launch_block8_few(*a, nullptr, &x->dev, x->dev.n, y, ctx->sm_count, ctx->stream));
+    if (x->dev.n <= ASP_BLOCK8_APPLY_ROWS) return launched(asp::launch_block8_few(*a, nullptr, &x->dev, x->dev.n, y, ctx->sm_count, ctx->fault, ctx->stream));
     return launched(asp::launch_block8_product(*a, x->dev, y, ctx->sm_count, ctx->fault, ctx->stream));
 }
 

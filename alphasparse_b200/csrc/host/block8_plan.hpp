@@ -6,9 +6,14 @@ namespace asp
 {
 namespace host
 {
-// Products with a few rows (k_block8_few): CTAs that share the blocks of a block row. Two CTAs fit an SM, and all run at once: with twice as many as fit
-// (8192 x 8192, one row, eight CTAs a block row) a call took 17.7 us instead of 13.2.
-unsigned block8_few_split(unsigned n_block_rows, unsigned longest, int sm_count);
+// CTAs that share work are a cluster of 1 to 8; fit[s]: how many clusters of s CTAs run at once, two CTAs an SM or one, as the kernel takes (ClusterRoom).
+// Those that do not fit would run after the others: 5000 x 5000, one row, 7 CTAs a block row, take 13.1 us, 6, which fit, 8.3.
+
+// Products with up to 32 rows: by the kernel for few rows or for a batch (k_block8_few, k_block8_batch)?
+bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, int sm_count);
+// and CTAs that share the blocks of a block row
+unsigned block8_few_split(unsigned n_block_rows, unsigned longest, const unsigned *fit);
+unsigned block8_batch_split(unsigned n_block_rows, unsigned longest, int sm_count, const unsigned *fit);
 
 // Products with many rows (k_block8_product): rows of X a tile (64, 128, 192), and CTAs that share the blocks of a tile (1 to 8).
 struct Block8ProductPlan
@@ -16,7 +21,7 @@ struct Block8ProductPlan
     unsigned tile, split;
 };
 constexpr unsigned kBlock8ProductRows = 192;
-Block8ProductPlan block8_product_plan(unsigned n_block_rows, unsigned n_blocks, unsigned longest, unsigned n, int sm_count);
+Block8ProductPlan block8_product_plan(unsigned n_block_rows, unsigned n_blocks, unsigned longest, unsigned n, int sm_count, const unsigned *fit);
 
 // Gradients (k_block8_gradient): blocks of a block column that share x at most (1, 2), and CTAs that share the rows of a group (1, 2, 4, 8).
 // blocks: stored ones; twos: groups of two where there are two at most.
@@ -25,7 +30,7 @@ struct Block8GradientPlan
     unsigned most, split;
 };
 constexpr unsigned kBlock8GradientRows = 64; // rows a step
-Block8GradientPlan block8_gradient_plan(unsigned blocks, unsigned twos, unsigned n, int sm_count);
+Block8GradientPlan block8_gradient_plan(unsigned blocks, unsigned twos, unsigned n, int sm_count, const unsigned *fit);
 } // namespace host
 } // namespace asp
 #endif

@@ -7,7 +7,6 @@
 
 #include <cooperative_groups.h>
 
-#include <type_traits>
 
 namespace asp
 {
@@ -36,12 +35,10 @@ template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const
     if (row >= n) return;
     Raw<T> raw;
     raw.load(x + (uint64_t)row * ld + blk * 128, x, x + (uint64_t)(n - 1) * ld + out.n_cols, lane8);
-    float v[16];
-    raw.floats(v, lane8, out.n_cols - min(out.n_cols, blk * 128)); // (zeros behind the last column, and behind the last block)
-    bool infinite;
-    const unsigned scale = scale_of_8(v, infinite);
+    uint4 u[Raw<T>::pieces];
+    raw.elements(u, lane8, out.n_cols - min(out.n_cols, blk * 128)); // (zeros behind the last column, and behind the last block)
     unsigned q[4];
-    pack16(v, scale, infinite, q);
+    const unsigned scale = to_eight<T>(u, q);
     if (blk < n_blocks) store_block<T>(q, lane8, out.values + (uint64_t)row * out.ld + blk * 128);
     unsigned four = scale << lane / 8 * 8;
     four |= __shfl_xor_sync(~0u, four, 8);
@@ -158,7 +155,7 @@ __global__ void __launch_bounds__(256) k_block8_get(const uint8_t *values, const
 
 // ---- products with a few rows ----------------------------------------------------------------------------------------
 
-// n <= 32 rows. Y[t][128 R + r] = sum over the blocks j of block row R of 2^(kA + kX) sum over c of A_j[r][c] X_j[t][c].
+// n <= 32 rows, a few blocks a CTA (block8_batch). Y[t][128 R + r] = sum over the blocks j of block row R of 2^(kA + kX) sum over c of A_j[r][c] X_j[t][c].
 //
 // The matrix is read once and nothing else counts: 16 KB a block, four or five blocks ahead, as the A operand of m16n8k16 with a warp to 16 rows (a
 // thread copies what it will itself read: no warp waits for another's); X in shared memory is the B operand, 8 rows of it a tile. Both as fp16, which has every e4m3 number: the form for e4m3 converts
@@ -172,9 +169,8 @@ __global__ void __launch_bounds__(256) k_block8_get(const uint8_t *values, const
 // X is converted for 4 / NT blocks at a time, which is a row's block to each eight lanes, and asked for while the stage before the one before is
 // multiplied: a stage's X is in shared memory, the next one's in registers.
 //
-// One row of bf16, all blocks stored: 8192 x 8192 in 13.0 us, 5.2 TB/s (and 23,000 x 23,000, where the start and the end count for less, at 6.5); 1024 x 1024 in 2.9,
-// which is a launch, X's conversion and the cluster's sum. 32 rows of 8192 x 8192 take 30 us: the products of a block, behind one another in
-// a warp, then take longer than its copy.
+// One row of bf16, half of 1024 x 1024: 3.1 us, of which the blocks are the least: a launch, X on its way and converted, the products, the cluster's sum. 4096 x 4096, all
+// of it: 6.0 us, 2.8 TB/s.
 constexpr int kFewPitch = 272; // bytes a row and block: 16-byte reads of 8 lanes in 2 rows meet no conflict
 template <int NT> constexpr int kFewAhead = NT == 4 ? 4 : 5; // blocks on their way: two CTAs' 128 or 160 KB an SM, with room for X
 template <int NT> struct FewShared
@@ -188,11 +184,10 @@ template <int NT> struct FewShared
 struct FewArgs
 {
     Block8Dev a;
-    Rows8Dev held;
-    const void *x;
+    XRows x;
     void *y;
-    uint64_t ldx, ldy;
-    unsigned n, n_split;
+    uint64_t ldy;
+    unsigned n_split;
 };
 
 __device__ __forceinline__ void mma_f16(float *c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
@@ -213,60 +208,24 @@ __device__ __forceinline__ void unpack16(uint4 q, unsigned *h)
     }
 }
 
-struct Held // X is in 8 bits already
+// eight lanes' part of a row's block to shared memory, as fp16 in the products' units
+template <class X> __device__ __forceinline__ unsigned put(const Fetched<X> &got, uint8_t *to, unsigned lane8, bool there) // (`there` or not, for the exchanges)
 {
-};
-// What eight lanes have of a row's block on its way to shared memory: as fp16 in the products' units, and the block's scale
-template <class X> struct Fetched
-{
-    Raw<X> raw;
-    unsigned columns; // of the block that are in the row
-    __device__ __forceinline__ void ask(const FewArgs &args, uint64_t row, unsigned kb, unsigned lane8)
-    {
-        const X *x = reinterpret_cast<const X *>(args.x);
-        columns = args.a.n_cols - kb * 128;
-        raw.load(x + row * args.ldx + kb * 128, x, x + (args.n - 1) * args.ldx + args.a.n_cols, lane8);
-    }
-    __device__ __forceinline__ unsigned put(uint8_t *to, unsigned lane8, bool there) const // (`there` or not, for the exchanges)
-    {
-        float v[16];
-        raw.floats(v, lane8, columns);
-        bool infinite;
-        const unsigned scale = scale_of_8(v, infinite);
-        unsigned q[4], h[8];
-        pack16(v, scale, infinite, q);
-        unpack16(make_uint4(q[0], q[1], q[2], q[3]), h);
-        if (!there) return scale;
-        constexpr int per = 16 / sizeof(X);
+    unsigned q[4], h[8];
+    const unsigned scale = got.eight(q, lane8);
+    if (!there) return scale;
+    unpack16(make_uint4(q[0], q[1], q[2], q[3]), h);
 #pragma unroll
-        for (int i = 0; i < 16; i += per)
-        {
-            uint8_t *at = to + 2 * column_in_block<X>(i, lane8);
-            if constexpr (per == 4) *reinterpret_cast<uint2 *>(at) = make_uint2(h[i / 2], h[i / 2 + 1]);
-            else *reinterpret_cast<uint4 *>(at) = make_uint4(h[i / 2], h[i / 2 + 1], h[i / 2 + 2], h[i / 2 + 3]);
-        }
-        return scale;
-    }
-};
-template <> struct Fetched<Held>
-{
-    uint4 q;
-    unsigned scale;
-    __device__ __forceinline__ void ask(const FewArgs &args, uint64_t row, unsigned kb, unsigned lane8)
+    for (int i = 0; i < 16; i += Fetched<X>::per)
     {
-        q = *reinterpret_cast<const uint4 *>(args.held.values + row * args.held.ld + kb * 128 + 16 * lane8);
-        scale = args.held.scales[scale_at(args.held, row, kb)];
+        uint8_t *at = to + 2 * Fetched<X>::column(i, lane8);
+        if constexpr (Fetched<X>::per == 4) *reinterpret_cast<uint2 *>(at) = make_uint2(h[i / 2], h[i / 2 + 1]);
+        else
+#pragma unroll
+            for (int k = 0; k < Fetched<X>::per / 2; k += 4) *reinterpret_cast<uint4 *>(at + 4 * k) = make_uint4(h[i / 2 + k], h[i / 2 + k + 1], h[i / 2 + k + 2], h[i / 2 + k + 3]);
     }
-    __device__ __forceinline__ unsigned put(uint8_t *to, unsigned lane8, bool there) const // (`there` or not, for the exchanges)
-    {
-        if (!there) return scale;
-        unsigned h[8];
-        unpack16(q, h);
-        *reinterpret_cast<uint4 *>(to + 32 * lane8) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4 *>(to + 32 * lane8 + 16) = make_uint4(h[4], h[5], h[6], h[7]);
-        return scale;
-    }
-};
+    return scale;
+}
 
 template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_block8_few(const FewArgs args)
 {
@@ -276,7 +235,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     const cg::cluster_group cluster = cg::this_cluster();
     const unsigned split = args.n_split, piece = blockIdx.x % split;
     const uint4 mine_of = args.a.rows[blockIdx.x / split];
-    const unsigned tokens = args.n, br = mine_of.x, lo = mine_of.y, len = mine_of.z;
+    const unsigned tokens = args.x.n, br = mine_of.x, lo = mine_of.y, len = mine_of.z;
     const unsigned j0 = lo + (unsigned)((uint64_t)len * piece / split), j1 = lo + (unsigned)((uint64_t)len * (piece + 1) / split);
     const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
 
@@ -336,25 +295,25 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     unsigned block_scale = 127;
     const auto ask = [&](unsigned j) { // of the stage that begins with block j
         if (j + slot >= j1 || t >= tokens) return;
-        got.ask(args, t, args.a.col[j + slot], lane8);
+        got.ask(args.x, t, args.a.col[j + slot], lane8);
         block_scale = args.a.scales[j + slot];
     };
-    const auto put = [&](unsigned j) {
+    const auto convert = [&](unsigned j) {
         const unsigned at = (j - j0) / per % 2;
         const bool there = j + slot < j1 && t < tokens;
-        const unsigned both = got.put(sh.x[at][slot][t], lane8, there) + block_scale, half = both / 2; // exponents + 127 each
+        const unsigned both = put(got, sh.x[at][slot][t], lane8, there) + block_scale, half = both / 2; // exponents + 127 each
         if (there && lane8 == 0) sh.factor[at][slot][t] = make_float2(power(half), power(both - half));
     };
     ask(j0);
     __syncthreads(); // (zeros everywhere)
-    put(j0);
+    convert(j0);
     ask(j0 + per);
     for (unsigned j = j0; j < j1; j += per)
     {
         __syncthreads();
         if (j + per < j1) // (the same for all of the CTA)
         {
-            put(j + per);
+            convert(j + per);
             ask(j + 2 * per);
         }
         for (unsigned k = j; k < min(j + per, j1); k++)
@@ -387,19 +346,23 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     cluster.sync(); // (its shared memory is read until here)
 }
 
-template <int NT, class X, class Y> cudaError_t few(const FewArgs &args, cudaStream_t st)
+template <int NT, class X, class Y> cudaError_t few(FewArgs &args, cudaStream_t st)
 {
     auto *kernel = k_block8_few<NT, X, Y>;
     const size_t smem = sizeof(FewShared<NT>);
     static SharedAllowance allowance;
-    const cudaError_t e = allowance.need((const void *)kernel, (int)smem);
+    static ClusterRoom room;
+    unsigned fit[9];
+    cudaError_t e = allowance.need((const void *)kernel, (int)smem);
+    if (e == cudaSuccess) e = room.most((const void *)kernel, 256, smem, fit);
     if (e != cudaSuccess) return e;
+    args.n_split = host::block8_few_split(args.a.n_block_rows, args.a.longest, fit);
     return launch_pdl_cluster(kernel, args.n_split, dim3(args.a.n_block_rows * args.n_split), dim3(256), smem, st, args);
 }
-template <class X, class Y> cudaError_t few_by_rows(const FewArgs &args, cudaStream_t st)
+template <class X, class Y> cudaError_t few_by_rows(FewArgs &args, cudaStream_t st)
 {
-    if (args.n <= 8) return few<1, X, Y>(args, st);
-    if (args.n <= 16) return few<2, X, Y>(args, st);
+    if (args.x.n <= 8) return few<1, X, Y>(args, st);
+    if (args.x.n <= 16) return few<2, X, Y>(args, st);
     return few<4, X, Y>(args, st);
 }
 } // namespace
@@ -439,24 +402,23 @@ cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st)
     return launch_pdl(k_block8_get, dim3(a.n_blocks * 4), dim3(256), 0, st, a.values, a.scales, out);
 }
 
-cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, cudaStream_t st)
+cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st)
 {
     if (n == 0) return cudaSuccess;
+    if (host::block8_batch(a.n_block_rows, a.longest, n, sm_count)) return launch_block8_batch(a, x, held, n, y, sm_count, fault, st);
     FewArgs args = {};
     args.a = a;
-    args.n = n;
+    args.x.n = n, args.x.n_cols = a.n_cols;
     args.y = y.p;
     args.ldy = y.ld;
-    args.n_split = host::block8_few_split(a.n_block_rows, a.longest, sm_count);
     return by_type(y.dtype, [&](auto ty) {
         using Y = decltype(ty);
         if (held)
         {
-            args.held = *held;
+            args.x.held = *held;
             return few_by_rows<Held, Y>(args, st);
         }
-        args.x = x->p;
-        args.ldx = x->ld;
+        args.x.p = x->p, args.x.ld = x->ld;
         return by_type(x->dtype, [&](auto tx) {
             using X = decltype(tx);
             return few_by_rows<X, Y>(args, st);

@@ -44,6 +44,7 @@ constexpr unsigned kHeld = 4, kHeldBytes = kTile + 1024;      // x in 8 bits, an
 static_assert(kHeld % 2 == 0, "places for x are shared out between two groups of warps");
 constexpr unsigned kUnfolded = 3, kUnfoldedBytes = 2 * kTile; // x in 16 bits: 64 columns after 64 columns, a row t 128 bytes
 constexpr unsigned kThreads = 896;
+constexpr size_t kSharedBytes = kRoom * kBlockBytes + kUnfolded * kUnfoldedBytes + kHeld * kHeldBytes + 1024;
 // Rows of dy that are not all on 16-byte boundaries cannot be copied by tiles. The warps that unfold x bring them, one of their steps ahead, in the aligned
 // pieces of 16 bytes that they lie in, and shift them to where they belong: 4001 rows, a quarter of 4001 x 4003, take 133 us (450 element by
 // element) where 4096 rows of 4096 x 4096 take 42 by tiles. They then take a part of dy's room, and groups are single blocks.
@@ -470,12 +471,11 @@ end:
 
 template <class Unfold> cudaError_t gradient(const CUtensorMap &map_dy, const CUtensorMap &map_x, const GradientArgs &p, int sm_count, cudaStream_t st)
 {
-    const size_t smem = kRoom * kBlockBytes + kUnfolded * kUnfoldedBytes + kHeld * kHeldBytes + 1024;
     static SharedAllowance allowance;
-    const cudaError_t e = allowance.need((const void *)k_block8_gradient<Unfold>, (int)smem);
+    const cudaError_t e = allowance.need((const void *)k_block8_gradient<Unfold>, (int)kSharedBytes);
     if (e != cudaSuccess) return e;
     const unsigned grid = p.split > 1 ? p.n_groups * p.split : std::min<unsigned>(p.n_groups, (unsigned)sm_count);
-    return launch_pdl_cluster(k_block8_gradient<Unfold>, p.split, dim3(grid), dim3(kThreads), smem, st, map_dy, map_x, p);
+    return launch_pdl_cluster(k_block8_gradient<Unfold>, p.split, dim3(grid), dim3(kThreads), kSharedBytes, st, map_dy, map_x, p);
 }
 
 } // namespace
@@ -486,7 +486,14 @@ cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &group
     if (x.n == 0) return accumulate ? cudaSuccess : cudaMemsetAsync(out, 0, (size_t)a.n_blocks * 16384 * sizeof(float), st);
     GradientArgs p = {};
     const bool direct = ((uintptr_t)dy.p & 15) == 0 && dy.ld % 8 == 0 && dy.ld < 1ull << 38; // (a tile map's distances are below 2^40 bytes)
-    const host::Block8GradientPlan plan = host::block8_gradient_plan(a.n_blocks, direct ? groups.twos : 0, x.n, sm_count);
+    static SharedAllowance allowance;
+    static ClusterRoom room;
+    unsigned fit[9];
+    const void *any = (const void *)k_block8_gradient<UnfoldB16>; // (of both types, one CTA fits an SM)
+    cudaError_t e = allowance.need(any, (int)kSharedBytes);
+    if (e == cudaSuccess) e = room.most(any, kThreads, kSharedBytes, fit);
+    if (e != cudaSuccess) return e;
+    const host::Block8GradientPlan plan = host::block8_gradient_plan(a.n_blocks, direct ? groups.twos : 0, x.n, sm_count, fit);
     p.most = plan.most, p.split = plan.split;
     p.x = x, p.list = groups.groups[p.most - 1], p.n_groups = groups.count[p.most - 1];
     p.dy = dy.p, p.ld = dy.ld, p.out = out, p.accumulate = accumulate, p.fault = fault;
@@ -494,7 +501,7 @@ cudaError_t launch_block8_gradient(const Block8Dev &a, const Block8Groups &group
     p.stages = direct ? kRoom / p.most : kShiftedStages;
     p.direct = direct;
     CUtensorMap map_dy, map_x;
-    cudaError_t e = byte_map(&map_x, x.values, x.ld, x.n, x.ld, kRows, false); // as it lies, without swizzle
+    e = byte_map(&map_x, x.values, x.ld, x.n, x.ld, kRows, false); // as it lies, without swizzle
     if (e == cudaSuccess && p.direct)
         e = tensor_map(&map_dy, dy.dtype == ASP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dy.p, a.n_rows, x.n, dy.ld * 2, 64, kRows);
     else map_dy = map_x; // (not used)

@@ -42,7 +42,6 @@ constexpr unsigned kStages = 8; // at most
 constexpr unsigned kScaleBytes = 512 + 1024;
 constexpr unsigned kRoom = 221 * 1024; // of shared memory for stages
 constexpr unsigned kThreads = 320;
-constexpr uint64_t kNear = 40ull << 20;
 
 struct ProductArgs
 {
@@ -66,7 +65,8 @@ struct Shared
 };
 
 // The steps of a CTA, in order: the blocks of its tiles. Tiles are in the order of their block rows, longest first, and handed out to the CTAs forwards and backwards in
-// turn, so that who has a long one gets a short one next (a quarter of 4096 x 4096 by 2048 rows: SCHED_A us, SCHED_B with block rows side by side and always forwards).
+// turn, so that who has a long one gets a short one next (a quarter of 4096 x 4096 by 2048 rows: 17.8 us, 19.1 with block rows side by side and always
+// forwards). What a CTA has to know of a tile is asked for a tile ahead (17.8 to 17.0 us).
 // Where X is larger than a part of L2 it is gone through in parts of `wide` tiles, each with all block rows.
 struct Steps
 {
@@ -338,7 +338,7 @@ template <class Y> cudaError_t product(const CUtensorMap &map_a, const CUtensorM
 {
     const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
     static SharedAllowance allowance;
-    const cudaError_t e = allowance.need((const void *)k_block8_product<Y>, (int)smem);
+    const cudaError_t e = allowance.need((const void *)k_block8_product<Y>, kRoom + 1024);
     if (e != cudaSuccess) return e;
     const unsigned grid = p.split > 1 ? p.n_tiles * p.split : std::min<unsigned>(p.n_tiles, (unsigned)sm_count);
     return launch_pdl_cluster(k_block8_product<Y>, p.split, dim3(grid), dim3(kThreads), smem, st, map_a, map_x, p);
@@ -350,19 +350,25 @@ cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const D
     if (x.n == 0) return cudaSuccess;
     ProductArgs p = {};
     p.a = a, p.x = x, p.y = y.p, p.ldy = y.ld, p.fault = fault;
-    const host::Block8ProductPlan plan = host::block8_product_plan(a.n_block_rows, a.n_blocks, a.longest, x.n, sm_count);
+    static SharedAllowance allowance;
+    static ClusterRoom room;
+    unsigned fit[9];
+    const void *any = (const void *)k_block8_product<float>; // (of all types, one CTA fits an SM)
+    cudaError_t e = allowance.need(any, kRoom + 1024);
+    if (e == cudaSuccess) e = room.most(any, kThreads, kRoom + 1024, fit);
+    if (e != cudaSuccess) return e;
+    const host::Block8ProductPlan plan = host::block8_product_plan(a.n_block_rows, a.n_blocks, a.longest, x.n, sm_count, fit);
     p.tile = plan.tile, p.split = plan.split;
     p.tiles_x = (x.n + p.tile - 1) / p.tile;
     const uint64_t tiles = (uint64_t)a.n_block_rows * p.tiles_x;
     if (tiles > 0xf0000000u) return cudaErrorInvalidValue; // (2^38 rows of blocks' results and more)
     p.n_tiles = (unsigned)tiles;
-    // Tiles of X that are gone through together: all where X stays in L2 at hand (8192 x 8192 bytes do not), else so many that the tiles that run at the same time
-    // have as many bytes of A as of X.
+    // Tiles of X that are gone through together: all where X stays near in L2, else so many that the tiles that run at the same time have as many bytes of A as of X.
     p.wide = p.tiles_x;
-    if (x.n * x.ld > kNear)
+    if (x.n * x.ld > 40ull << 20) // 8192 rows of 8192: 4096 of them, a quarter, 76.3 us in parts and 81.5 without; 8192 rows of 4096 (34 MB) 89 and 88
     {
         const double side = 16384.0 * a.n_blocks / a.n_block_rows / (p.tile * x.ld);
-        const unsigned parts = (p.tiles_x + std::max(1u, (unsigned)(sqrt(sm_count * side) + 0.5)) - 1) / std::max(1u, (unsigned)(sqrt(sm_count * side) + 0.5));
+        const unsigned most = std::max(1u, (unsigned)(sqrt(sm_count * side) + 0.5)), parts = (p.tiles_x + most - 1) / most;
         p.wide = (p.tiles_x + parts - 1) / parts;
     }
     p.stage_bytes = (16384 + p.tile * 128 + kScaleBytes + 1023) / 1024 * 1024;
@@ -370,7 +376,7 @@ cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const D
     p.pairs = y.dtype != ASP_F32 && ((uintptr_t)y.p & 3) == 0 && y.ld % 2 == 0;
     CUtensorMap map_a, map_x;
     // (a matrix without blocks has nothing to copy: any map does)
-    cudaError_t e = byte_map(&map_a, a.values, 128, (uint64_t)std::max(1u, a.n_blocks) * 128, 128, 128);
+    e = byte_map(&map_a, a.values, 128, (uint64_t)std::max(1u, a.n_blocks) * 128, 128, 128);
     if (e == cudaSuccess) e = byte_map(&map_x, x.values, x.ld, x.n, x.ld, p.tile);
     if (e != cudaSuccess) return e;
     if (y.dtype == ASP_F32) return product<float>(map_a, map_x, p, sm_count, st);

@@ -70,6 +70,39 @@ class SharedAllowance
     }
 };
 
+// How many clusters of 1 to 8 CTAs of one kernel run at once: the parts of the chip have different numbers of SMs, so this is the driver's to say. Asked once
+// per device (after SharedAllowance::need).
+class ClusterRoom
+{
+    std::atomic<unsigned> known[64][9] = {};
+
+  public:
+    cudaError_t most(const void *kernel, unsigned threads, size_t smem, unsigned clusters[9])
+    {
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        for (unsigned s = 1; s <= 8 && e == cudaSuccess; s++)
+        {
+            if (device < 64 && (clusters[s] = known[device][s].load(std::memory_order_relaxed)) > 0) continue;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(s);
+            cfg.blockDim = dim3(threads);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute at;
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = s;
+            at.val.clusterDim.y = at.val.clusterDim.z = 1;
+            cfg.attrs = &at;
+            cfg.numAttrs = 1;
+            int n = 0;
+            e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+            clusters[s] = (unsigned)n;
+            if (e == cudaSuccess && device < 64) known[device][s].store(clusters[s], std::memory_order_relaxed);
+        }
+        return e;
+    }
+};
+
 template <class... A>
 cudaError_t launch_pdl_cluster(void (*kernel)(A...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
 {

@@ -118,6 +118,23 @@ def test_every_bf16_and_every_rounding(asp_ctx):
         held.close()
 
 
+def test_every_f16_with_neighbours_of_all_sizes(asp_ctx):
+    """All 65536 of them, NaN and infinite ones included: side by side, shuffled, and each among tiny ones (whose scales fp16 itself does not have)."""
+    every = torch.arange(0x10000, dtype=torch.int32).to(torch.int16).view(torch.float16)
+    shuffled = every[torch.randperm(0x10000, generator=torch.Generator().manual_seed(1))]
+    tiny = torch.arange(0x10000, dtype=torch.int32).remainder(16).to(torch.int16).view(torch.float16).reshape(-1, 128).repeat(8, 1)
+    tiny[:, 5] = torch.arange(tiny.shape[0], dtype=torch.int32).remainder(0x400).to(torch.int16).view(torch.float16)  # every subnormal one
+    for v in (every.reshape(-1, 128), shuffled.reshape(-1, 128), tiny, torch.zeros(3, 128, dtype=torch.float16)):
+        v = v.contiguous().cuda()
+        held, out = Rows8(asp_ctx, v.shape[0], 128), torch.empty(v.shape, device="cuda")
+        torch.cuda.synchronize()
+        held.quantize(v.data_ptr(), v.shape[0], "f16")
+        held.restore(out.data_ptr(), "f32")
+        asp_ctx.synchronize()
+        assert same(out, ref.rows_in_8_bits(v))
+        held.close()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_rows_that_are_not_finite(asp_ctx, dtype):
     x = rows(5, 6, 300, dtype)
@@ -250,6 +267,51 @@ def test_apply(asp_ctx, n, n_rows, n_cols, density, transposed):
     m.close()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n_rows,n_cols,density,pad,offset", [(300, 9000, 0.9, 0, 0), (2500, 3500, 0.8, 1, 0), (5000, 2600, 1.0, 0, 3), (130, 8195, 0.6, 5, 0)])
+@pytest.mark.parametrize("n", [1, 4, 8, 9, 16, 17, 20, 31, 32])
+def test_apply_to_long_block_rows(asp_ctx, n, n_rows, n_cols, density, pad, offset, dtype):
+    m, a = matrix(asp_ctx, n_rows + n, n_rows, n_cols, density, transposed=False, empty_row=1)
+    x = rows(n, n, n_cols, dtype, pad, offset)
+    ld = n_cols + pad
+    got = []
+    for y_dtype, y_pad in (("f32", 0), (dtype, 3), ("f32", 0)):
+        y = torch.full((n + 1, n_rows + y_pad), 7.0, dtype=TYPES[y_dtype], device="cuda")
+        torch.cuda.synchronize()
+        m.apply(x.data_ptr(), n, dtype, y.data_ptr(), y_dtype, ld, n_rows + y_pad)
+        asp_ctx.synchronize()
+        assert_sums(y[:n, :n_rows], ref.rows_in_8_bits(x), a, y_dtype, f"apply {n} {dtype} {y_dtype}")
+        assert (y[n] == 7.0).all() and (y[:, n_rows:] == 7.0).all()
+        got.append(y)
+    assert torch.equal(got[0], got[2])
+    # rows that are in 8 bits already go through the same kernels
+    held = Rows8(asp_ctx, n, n_cols)
+    held.quantize(x.data_ptr(), n, dtype, ld)
+    got[2].fill_(7.0)
+    torch.cuda.synchronize()
+    m.product(held, got[2].data_ptr(), "f32")
+    asp_ctx.synchronize()
+    assert torch.equal(got[0], got[2])
+    m.close()
+    held.close()
+
+
+@pytest.mark.parametrize("n", [2, 12, 30])
+def test_long_block_rows_and_rows_that_are_not_finite(asp_ctx, n):
+    m, a = matrix(asp_ctx, 4, 260, 6000, 1.0)
+    x = rows(2, n, 6000, "bf16")
+    x[1, 5], x[n - 1, 5999] = float("nan"), float("inf")
+    y = torch.full((n, 260), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    m.apply(x.data_ptr(), n, "bf16", y.data_ptr(), "f32")
+    asp_ctx.synchronize()
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[1] = bad[n - 1] = True
+    assert torch.equal(y.isnan().all(1), bad) and torch.equal(y.isnan().any(1), bad)
+    assert_sums(y[~bad], ref.rows_in_8_bits(x)[~bad], a, "f32", "the other rows")
+    m.close()
+
+
 @pytest.mark.parametrize("transposed", [False, True])
 @pytest.mark.parametrize("n_rows,n_cols,density", SHAPES)
 @pytest.mark.parametrize("n", [1, 31, 33, 100, 224, 225, 449, 1000])
@@ -376,6 +438,31 @@ def test_scales_far_apart(asp_ctx, n):
     asp_ctx.synchronize()
     a = ref.dense(m.pattern(), (128, 256), ref.groups_in_8_bits(values.reshape(2, -1)).reshape(2, 128, 128))
     assert_sums(y, ref.rows_in_8_bits(x), a, "f32", "far apart")
+
+
+@pytest.mark.parametrize("n,n_cols", [(4, 256), (4, 6016), (20, 6016), (200, 256)])
+@pytest.mark.parametrize("k", [70, -70])
+def test_scales_whose_product_no_32_bit_number_is(asp_ctx, n, n_cols, k):
+    """Two exponents that add up to 140 or -140, and products that 32 bits have: of elements far below (above) the largest of their blocks."""
+    blocks = n_cols // 128
+    m = Block8(asp_ctx, 128, n_cols, [0, blocks], list(range(blocks)))
+    values, x = torch.zeros(blocks, 128, 128, device="cuda"), torch.zeros(n, n_cols, device="cuda")
+    values[0, 0, 0] = x[:, 0] = 2.0 ** (k + 8)  # what makes the scale 2^k; their product, 2^(2 k + 16), is row 0
+    values[0, 1:, 1] = x[:, 1] = 2.0 ** (k - 6)
+    y, held = torch.empty(n, 128, device="cuda"), Rows8(asp_ctx, n, n_cols)
+    torch.cuda.synchronize()
+    m.set_values(values.data_ptr(), "f32")
+    if n <= 32:
+        m.apply(x.data_ptr(), n, "f32", y.data_ptr(), "f32")
+    else:
+        held.quantize(x.data_ptr(), n, "f32")
+        m.product(held, y.data_ptr(), "f32")
+    asp_ctx.synchronize()
+    want = torch.full((n, 128), 4.0 ** (k - 6), dtype=torch.float64, device="cuda")
+    want[:, 0] = 4.0 ** (k + 8)
+    assert torch.equal(y, want.float())
+    m.close()
+    held.close()
 
 
 # ---- gradients -------------------------------------------------------------------------------------------------------
