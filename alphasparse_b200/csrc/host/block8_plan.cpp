@@ -23,10 +23,12 @@ unsigned largest(unsigned n_block_rows, unsigned longest, unsigned ctas, const u
 // warps) costs 0.7 us more. One row: 4096 x 4096 (4 blocks a CTA) 6.0 us by the kernel for few rows and 6.2 by that for a batch, 2048 x 8192, half of it (5), 6.0 and 5.6,
 // 8192 x 8192 (16) 13.6 and 9.9. With more than 8 rows mma.sync takes longer than the blocks to come: 16 rows of 4096 x 4096 8.4 and 7.5, of 4001 x 2047 in 32 bits
 // (2) 6.0 and 7.0, 32 rows of 8192 x 8192 31.2 and 17.6, of 1024 x 1024 (1) 4.4 and 5.2.
-bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, int sm_count)
+// wide: the result has 32 bits. A sum of the kernel for a batch is all of a CTA's blocks, cut off each time something is added (16 blocks: 6e-7); the other one rounds
+// after each block.
+bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, bool wide, int sm_count)
 {
-    const unsigned split = std::max(1u, std::min(8u, 2u * (unsigned)sm_count / n_block_rows));
-    return (longest + split - 1) / split >= (n <= 8 ? 5 : 3);
+    const unsigned split = std::max(1u, std::min(8u, 2u * (unsigned)sm_count / n_block_rows)), blocks = (longest + split - 1) / split;
+    return blocks >= (n <= 8 ? 5 : 3) && !(wide && blocks > kBlock8Sum);
 }
 
 unsigned block8_few_split(unsigned n_block_rows, unsigned longest, const unsigned *fit) { return largest(n_block_rows, longest, ~0u, fit); }

@@ -9,8 +9,11 @@ namespace host
 // CTAs that share work are a cluster of 1 to 8; fit[s]: how many clusters of s CTAs run at once, two CTAs an SM or one, as the kernel takes (ClusterRoom).
 // Those that do not fit would run after the others: 5000 x 5000, one row, 7 CTAs a block row, take 13.1 us, 6, which fit, 8.3.
 
+// Blocks in one sum of a tensor core, where the result has 32 bits
+constexpr unsigned kBlock8Sum = 16;
+
 // Products with up to 32 rows: by the kernel for few rows or for a batch (k_block8_few, k_block8_batch)?
-bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, int sm_count);
+bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, bool wide, int sm_count);
 // and CTAs that share the blocks of a block row
 unsigned block8_few_split(unsigned n_block_rows, unsigned longest, const unsigned *fit);
 unsigned block8_batch_split(unsigned n_block_rows, unsigned longest, int sm_count, const unsigned *fit);

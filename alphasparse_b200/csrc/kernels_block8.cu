@@ -405,7 +405,7 @@ cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st)
 cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st)
 {
     if (n == 0) return cudaSuccess;
-    if (host::block8_batch(a.n_block_rows, a.longest, n, sm_count)) return launch_block8_batch(a, x, held, n, y, sm_count, fault, st);
+    if (host::block8_batch(a.n_block_rows, a.longest, n, y.dtype == ASP_F32, sm_count)) return launch_block8_batch(a, x, held, n, y, sm_count, fault, st);
     FewArgs args = {};
     args.a = a;
     args.x.n = n, args.x.n_cols = a.n_cols;

@@ -23,7 +23,7 @@ using namespace block8;
 //
 // A tile is 128 rows of A by up to 192 rows of X: D[128][192] in tensor memory, a block of A (16 KB) and the same 128 columns of X (24 KB) a
 // step, four tcgen05.mma of 32 columns each. The powers of two go into the products as their scales (a byte per row of the block and per row of X), so sums
-// over blocks of different scales stay in tensor memory, in 32 bits, from the first block to the last. A's rows are the
+// over blocks of different scales stay in tensor memory, in 32 bits. A's rows are the
 // rows of D because a block is 128 rows of A whatever the pattern, while X can be cut anywhere; 192 since two tiles' sums (384
 // columns) and the scales (24) then share the 512 columns, so that a tile is stored under the next one's products, and whole 64s since the
 // scales of X begin at every second column.
@@ -36,12 +36,16 @@ using namespace block8;
 // power limit and 1.28 GHz, and it takes 303. 4096, 4096, 2048, a quarter: 18 us, 0.95 PFLOP/s (512 tiles over 148 SMs, the last wave half empty,
 // and each CTA's first copies and last stores).
 //
-// A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 9 store.
+// A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 17 store.
 constexpr unsigned kMostRows = host::kBlock8ProductRows;
 constexpr unsigned kStages = 8; // at most
+// Tensor cores cut off what they add up to: 64 blocks (8192 columns) in one sum were 3.0e-6 off, 16 are 6e-7, where sums rounded in 32 bits are 4e-7. Results in
+// 32 bits therefore take sums of 16 blocks, in one D and the other, added up, rounded, in the registers of the warps that store (2048 rows by 4096 x 8192: 70.4 us instead
+// of 68.3; added up by L2 where the result is: 83). In 16 bits, which lose 2^-9 or 2^-12 at the end, a hundredth of that is enough.
+template <class Y> constexpr unsigned kRound = sizeof(Y) == 4 ? host::kBlock8Sum : 256;
 constexpr unsigned kScaleBytes = 512 + 1024;
 constexpr unsigned kRoom = 221 * 1024; // of shared memory for stages
-constexpr unsigned kThreads = 320;
+constexpr unsigned kThreads = 576;
 
 struct ProductArgs
 {
@@ -104,6 +108,7 @@ struct Steps
     }
 };
 
+// 16 columns of D (rows of Y), 32 of its lanes
 template <class Y> __device__ __forceinline__ void store_columns(const float *v, const ProductArgs &p, unsigned row0, unsigned lane, unsigned t0, unsigned limit)
 {
     Y *y = reinterpret_cast<Y *>(p.y);
@@ -117,7 +122,7 @@ template <class Y> __device__ __forceinline__ void store_columns(const float *v,
             Y *to = y + (uint64_t)(t0 + odd) * p.ldy + (row & ~1u);
             const bool both = (row & ~1u) + 1 < p.a.n_rows, one = (row & ~1u) < p.a.n_rows;
 #pragma unroll
-            for (int c = 0; c < 32; c += 2)
+            for (int c = 0; c < 16; c += 2)
             {
                 const float got = __shfl_xor_sync(~0u, odd ? v[c] : v[c + 1], 1);
                 const Y lo = from_float<Y>(odd ? got : v[c]), hi = from_float<Y>(odd ? v[c + 1] : got);
@@ -137,7 +142,7 @@ template <class Y> __device__ __forceinline__ void store_columns(const float *v,
     }
     if (row >= p.a.n_rows) return;
 #pragma unroll
-    for (int c = 0; c < 32; c++)
+    for (int c = 0; c < 16; c++)
         if (t0 + c < limit) y[(uint64_t)(t0 + c) * p.ldy + row] = from_float<Y>(v[c]);
 }
 
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
         for (int i = 0; i < 2; i++)
         {
             tc::barrier_init(&sh.done[i], 1);
-            tc::barrier_init(&sh.taken[i], 8);
+            tc::barrier_init(&sh.taken[i], 16);
         }
         sh.gave_up = 0;
         tc::fence_barrier_init();
@@ -206,84 +211,92 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
             bool ready = false;
             for (; at.valid; at.next_tile())
             {
-                if (at.j == at.end) continue;
-                if (!tc::barrier_wait(&sh.taken[b], b_phase ^ 1, &sh.gave_up)) goto end;
-                const unsigned d = tensor + b * kMostRows, shift = at.t0 % 128 / 32; // (of the first row among its piece's columns)
-                bool add = false;
-                for (; at.j < at.end; at.j++)
+                const unsigned shift = at.t0 % 128 / 32; // (of the first row among its piece's columns)
+                while (at.j < at.end)
                 {
-                    const unsigned shape = tc::scaled_e4m3(p.tile, p.a.col[at.j] % 4);
-                    if (!ready && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
-                    tc::fence_after();
-                    const unsigned a = tc::shared_address(stages + s * p.stage_bytes), x = a + 16384, scales = x + x_bytes;
-                    const unsigned sa = tensor + 2 * kMostRows + turn * 4, sx = tensor + 2 * kMostRows + 8 + turn * 8;
-                    uint64_t *const empty = &sh.empty[s];
-                    if (++s == p.stages) s = 0, phase ^= 1;
-                    tc::copy_scales(sa, tc::scale_rows(scales));
-                    tc::copy_scales(sx, tc::scale_rows(scales + 512));
-                    if (shift + p.tile / 32 > 4) tc::copy_scales(sx + 4, tc::scale_rows(scales + 1024));
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
+                    if (!tc::barrier_wait(&sh.taken[b], b_phase ^ 1, &sh.gave_up)) goto end;
+                    const unsigned d = tensor + b * kMostRows, last = min(at.end, at.j + kRound<Y>);
+                    bool add = false;
+                    for (; at.j < last; at.j++)
                     {
-                        if (k == 1)
+                        const unsigned shape = tc::scaled_e4m3(p.tile, p.a.col[at.j] % 4);
+                        if (!ready && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
+                        tc::fence_after();
+                        const unsigned a = tc::shared_address(stages + s * p.stage_bytes), x = a + 16384, scales = x + x_bytes;
+                        const unsigned sa = tensor + 2 * kMostRows + turn * 4, sx = tensor + 2 * kMostRows + 8 + turn * 8;
+                        uint64_t *const empty = &sh.empty[s];
+                        if (++s == p.stages) s = 0, phase ^= 1;
+                        tc::copy_scales(sa, tc::scale_rows(scales));
+                        tc::copy_scales(sx, tc::scale_rows(scales + 512));
+                        if (shift + p.tile / 32 > 4) tc::copy_scales(sx + 4, tc::scale_rows(scales + 1024));
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
                         {
-                            ready = at.j + 1 < at.end;
-                            if (ready && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
+                            if (k == 1)
+                            {
+                                ready = at.j + 1 < at.end;
+                                if (ready && !tc::barrier_wait(&sh.full[s], phase, &sh.gave_up)) goto end;
+                            }
+                            tc::mma_scaled(d, tc::rows_k_major(a + 32 * k), tc::rows_k_major(x + 32 * k), shape, sa, sx + shift, add);
+                            add = true;
                         }
-                        tc::mma_scaled(d, tc::rows_k_major(a + 32 * k), tc::rows_k_major(x + 32 * k), shape, sa, sx + shift, add);
-                        add = true;
+                        tc::commit(empty);
+                        turn ^= 1;
                     }
-                    tc::commit(empty);
-                    turn ^= 1;
+                    tc::commit(&sh.done[b]);
+                    b ^= 1;
+                    if (b == 0) b_phase ^= 1;
                 }
-                tc::commit(&sh.done[b]);
-                b ^= 1;
-                if (b == 0) b_phase ^= 1;
             }
         }
     }
     else
     {
         unsigned b = 0, b_phase = 0;
-        const unsigned quarter = warp % 4, first = (warp - 2) / 4 * 32; // two warps to a quarter of D's lanes, every second 32 columns each
+        const unsigned quarter = warp % 4, first = (warp - 2) / 4 * 16; // four warps to a quarter of D's lanes, every fourth 16 columns each
+        constexpr unsigned most = kMostRows / 64;
         for (; at.valid; at.next_tile())
         {
             const unsigned row0 = at.row * 128 + quarter * 32, limit = min(p.x.n, at.t0 + p.tile);
-            float v[32];
-            if (p.split > 1)
+            float sum[most][16];
+#pragma unroll
+            for (unsigned k = 0; k < most; k++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) sum[k][i] = 0.f;
+            bool all = true;
+            while (at.j < at.end)
             {
-                // all blocks have been copied and multiplied: the stages are free
-                float *part = reinterpret_cast<float *>(stages) + quarter * 32 + lane;
-                const bool any = at.j < at.end;
-                if (any && !tc::barrier_wait(&sh.done[0], 0, &sh.gave_up)) break;
+                all = tc::barrier_wait<64>(&sh.done[b], b_phase, &sh.gave_up);
+                if (!all) break;
                 tc::fence_after();
-                for (unsigned c = first; c < p.tile; c += 64)
-                {
-                    if (any) tc::tensor_load32(tensor + c + (quarter * 32 << 16), v);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) part[(c + i) * 128] = any ? v[i] : 0.f;
-                }
-                break;
-            }
-            if (at.j == at.end)
-            {
+                for (unsigned k = 0; k < most; k++)
+                    if (first + 64 * k < p.tile)
+                    {
+                        float v[16];
+                        tc::tensor_load16(tensor + b * kMostRows + first + 64 * k + (quarter * 32 << 16), v);
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = 0.f;
-                for (unsigned c = first; c < p.tile; c += 64) store_columns<Y>(v, p, row0, lane, at.t0 + c, limit);
-                continue;
+                        for (int i = 0; i < 16; i++) sum[k][i] += v[i];
+                    }
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::barrier_arrive(&sh.taken[b]);
+                b ^= 1;
+                if (b == 0) b_phase ^= 1;
+                at.j += min(at.end - at.j, kRound<Y>);
             }
-            if (!tc::barrier_wait<64>(&sh.done[b], b_phase, &sh.gave_up)) break;
-            tc::fence_after();
-            for (unsigned c = first; c < p.tile; c += 64)
+            if (!all) break;
+            // a cluster's part goes to shared memory: all blocks have been copied and multiplied, the stages are free
+#pragma unroll
+            for (unsigned k = 0; k < most; k++)
             {
-                tc::tensor_load32(tensor + b * kMostRows + c + (quarter * 32 << 16), v);
-                store_columns<Y>(v, p, row0, lane, at.t0 + c, limit);
+                const unsigned c = first + 64 * k;
+                if (c >= p.tile) break;
+                if (p.split == 1) store_columns<Y>(sum[k], p, row0, lane, at.t0 + c, limit);
+                else
+#pragma unroll
+                    for (int i = 0; i < 16; i++) reinterpret_cast<float *>(stages)[(c + i) * 128 + quarter * 32 + lane] = sum[k][i];
             }
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::barrier_arrive(&sh.taken[b]);
-            b ^= 1;
-            if (b == 0) b_phase ^= 1;
         }
     }
 end:

@@ -395,6 +395,27 @@ def test_product_in_tiles_of_all_sizes(asp_ctx, n, n_rows, n_cols):
     held.close()
 
 
+@pytest.mark.parametrize("n,n_rows", [(40, 100), (300, 2000), (20, 200), (20, 5000)])
+def test_long_sums_in_32_bits_are_rounded(asp_ctx, n, n_rows):
+    """128 blocks, products of one sign. A tensor core cuts off less than 2^-23 of the sum each time it adds (32 columns): over 16 blocks, 64 times, to a sum that
+    grows evenly, less than 32.5 * 2^-23 in all, and eight such sums are added up with half a step each, 4 * 2^-23. (All 512 additions in one sum, of which half
+    a step is cut off on average, would come to 128 * 2^-23.)"""
+    m = Block8(asp_ctx, n_rows, 16384, *pattern(1, n_rows, 16384, 1.0))
+    values = torch.rand(m.n_blocks, 128, 128, generator=gen(1), device="cuda") + 0.5
+    x, held = torch.rand(n, 16384, generator=gen(2), device="cuda") + 0.5, Rows8(asp_ctx, n, 16384)
+    y = torch.empty(n, n_rows, device="cuda")
+    torch.cuda.synchronize()
+    m.set_values(values.data_ptr(), "f32")
+    held.quantize(x.data_ptr(), n, "f32")
+    m.product(held, y.data_ptr(), "f32")
+    asp_ctx.synchronize()
+    a = ref.dense(m.pattern(), (n_rows, 16384), ref.groups_in_8_bits(values.reshape(m.n_blocks, -1)).reshape(-1, 128, 128))
+    want = ref.rows_in_8_bits(x) @ a.T
+    assert ((y.double() - want).abs() / want).max().item() < (32.5 + 4) * 2.0**-23
+    m.close()
+    held.close()
+
+
 @pytest.mark.parametrize("n", [7, 20, 100, 400])
 def test_rows_that_are_not_finite_keep_it_to_themselves(asp_ctx, n):
     m, a = matrix(asp_ctx, 78, 700, 900, 1.0)
