@@ -92,7 +92,10 @@ class Block8:
 
     def __init__(self, ctx: capi.Context, n_rows: int, n_cols: int, block_ptr, block_col, transposed: bool = False):
         ptr = np.ascontiguousarray(block_ptr, dtype=np.int64)
-        col = np.ascontiguousarray(block_col, dtype=np.uint32)
+        col = np.asarray(block_col)
+        if col.size and (col.min() < 0 or col.max() >= 2**32):
+            raise ValueError("block_col: block columns")
+        col = np.ascontiguousarray(col, dtype=np.uint32)
         if ptr.ndim != 1 or ptr.shape[0] != -(-n_rows // BLOCK) + 1 or col.ndim != 1 or (ptr[-1] != col.shape[0]):
             raise ValueError("block_ptr has an entry for each block row and one more, the last of them the number of blocks")
         h = C.c_void_p()

@@ -57,7 +57,9 @@ cudaError_t launch_block8_set(const Block8Dev &a, const unsigned *row, const uns
 cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st);
 // a few rows, up to 32: X as it is (held == NULL) or in 8 bits. fault: a word that a kernel sets when it gives up a wait
 cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st);
-cudaError_t launch_block8_batch(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st);
+// fit: of block8_batch_room, the clusters of its kernel that run at once
+cudaError_t block8_batch_room(unsigned fit[9]);
+cudaError_t launch_block8_batch(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, const unsigned *fit, unsigned *fault, cudaStream_t st);
 // many rows in 8 bits
 cudaError_t launch_block8_product(const Block8Dev &a, const Rows8Dev &x, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st);
 // The blocks by block column, in groups (Block8Pattern): everything about a group in one place, since each look-up waits for the one before

@@ -19,18 +19,6 @@ unsigned largest(unsigned n_block_rows, unsigned longest, unsigned ctas, const u
 }
 } // namespace
 
-// Where a CTA has many blocks tcgen05 takes them as fast as they come, while its start (tensor memory, barriers, a step's way through three kinds of
-// warps) costs 0.7 us more. One row: 4096 x 4096 (4 blocks a CTA) 6.0 us by the kernel for few rows and 6.2 by that for a batch, 2048 x 8192, half of it (5), 6.0 and 5.6,
-// 8192 x 8192 (16) 13.6 and 9.9. With more than 8 rows mma.sync takes longer than the blocks to come: 16 rows of 4096 x 4096 8.4 and 7.5, of 4001 x 2047 in 32 bits
-// (2) 6.0 and 7.0, 32 rows of 8192 x 8192 31.2 and 17.6, of 1024 x 1024 (1) 4.4 and 5.2.
-// wide: the result has 32 bits. A sum of the kernel for a batch is all of a CTA's blocks, cut off each time something is added (16 blocks: 6e-7); the other one rounds
-// after each block.
-bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, bool wide, int sm_count)
-{
-    const unsigned split = std::max(1u, std::min(8u, 2u * (unsigned)sm_count / n_block_rows)), blocks = (longest + split - 1) / split;
-    return blocks >= (n <= 8 ? 5 : 3) && !(wide && blocks > kBlock8Sum);
-}
-
 unsigned block8_few_split(unsigned n_block_rows, unsigned longest, const unsigned *fit) { return largest(n_block_rows, longest, ~0u, fit); }
 
 // One CTA an SM where its blocks are few (16 rows of 4096 x 4096: 8 blocks to each of 128 CTAs 7.5 us, 4 to each of 256 8.2), two where they are many (one row of 8192 x 8192:
@@ -39,6 +27,18 @@ unsigned block8_batch_split(unsigned n_block_rows, unsigned longest, int sm_coun
 {
     const unsigned one = largest(n_block_rows, longest, (unsigned)sm_count, fit);
     return (longest + one - 1) / one <= 8 ? one : largest(n_block_rows, longest, ~0u, fit);
+}
+
+// Where a CTA has many blocks tcgen05 takes them as fast as they come, while its start (tensor memory, barriers, a step's way through three kinds of
+// warps) costs 0.7 us more. One row: 4096 x 4096 (4 blocks a CTA) 6.0 us by the kernel for few rows and 6.2 by that for a batch, 2048 x 8192, half of it (5), 6.0 and 5.6,
+// 8192 x 8192 (16) 13.6 and 9.9. With more than 8 rows mma.sync takes longer than the blocks to come: 16 rows of 4096 x 4096 8.4 and 7.5, of 4001 x 2047 in 32 bits
+// (2) 6.0 and 7.0, 32 rows of 8192 x 8192 31.2 and 17.6, of 1024 x 1024 (1) 4.4 and 5.2.
+// wide: the result has 32 bits. A sum of the kernel for a batch is all of a CTA's blocks, cut off each time something is added (16 blocks: 6e-7); the other one rounds
+// after each block.
+bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, bool wide, int sm_count, const unsigned *fit)
+{
+    const unsigned most = largest(n_block_rows, longest, ~0u, fit), split = block8_batch_split(n_block_rows, longest, sm_count, fit);
+    return (longest + most - 1) / most >= (n <= 8 ? 5 : 3) && !(wide && (longest + split - 1) / split > kBlock8Sum);
 }
 
 // A step takes as long as its 16 KB of A and its rows of X take to pass shared memory twice, at 128 bytes a clock; a tile costs some 2500 clocks beside

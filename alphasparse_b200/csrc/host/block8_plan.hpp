@@ -13,7 +13,7 @@ namespace host
 constexpr unsigned kBlock8Sum = 16;
 
 // Products with up to 32 rows: by the kernel for few rows or for a batch (k_block8_few, k_block8_batch)?
-bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, bool wide, int sm_count);
+bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, bool wide, int sm_count, const unsigned *fit);
 // and CTAs that share the blocks of a block row
 unsigned block8_few_split(unsigned n_block_rows, unsigned longest, const unsigned *fit);
 unsigned block8_batch_split(unsigned n_block_rows, unsigned longest, int sm_count, const unsigned *fit);

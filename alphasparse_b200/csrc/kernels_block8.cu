@@ -24,7 +24,7 @@ template <class F> cudaError_t by_type(int dtype, F f)
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
 // A row's four blocks to a warp, 8 lanes and 16 elements a lane each, so that an element is read once, its block's largest is known after
-// three exchanges, and the four scales leave as a word. Bounded by memory: 8192 x 8192 bf16 in 33.7 us, 202 MB at 6.0 TB/s. Eight rows to a CTA: no
+// three exchanges, and the four scales leave as a word. Bounded by memory: 8192 x 8192 bf16 in 32.8 us, 202 MB at 6.2 TB/s. Eight rows to a CTA: no
 // warp waits for another. Rows that begin anywhere cost the shifts: 4096 x 4001 bf16 in 11.8 us (8.7 for 4096 x 4096).
 template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const T *x, uint64_t ld, unsigned n, Rows8Dev out)
 {
@@ -46,7 +46,7 @@ template <class T> __global__ void __launch_bounds__(256) k_rows8_quantize(const
     if (lane == 0) *reinterpret_cast<unsigned *>(out.scales + scale_at(out, row, blk0)) = four; // (those behind the last block are not used)
 }
 
-// The same the other way: 8192 x 4096 to bf16 in 15.2 us, 101 MB at 6.6 TB/s (part of the 34 MB read still in L2); 4096 x 4001 in 15.6, as the ends of a warp's part
+// The same the other way: 8192 x 4096 to bf16 in 17 us, 101 MB at 5.9 TB/s; 4096 x 4001 in 15.6, as the ends of a warp's part
 // of a row are stored element by element. Registers are held down so that 48 (32 bits) or 64 (16 bits) warps fit an SM.
 template <class T> __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 6) k_rows8_restore(Rows8Dev x, T *out, uint64_t ld)
 {
@@ -405,7 +405,10 @@ cudaError_t launch_block8_get(const Block8Dev &a, float *out, cudaStream_t st)
 cudaError_t launch_block8_few(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st)
 {
     if (n == 0) return cudaSuccess;
-    if (host::block8_batch(a.n_block_rows, a.longest, n, y.dtype == ASP_F32, sm_count)) return launch_block8_batch(a, x, held, n, y, sm_count, fault, st);
+    unsigned fit[9];
+    const cudaError_t e = block8_batch_room(fit);
+    if (e != cudaSuccess) return e;
+    if (host::block8_batch(a.n_block_rows, a.longest, n, y.dtype == ASP_F32, sm_count, fit)) return launch_block8_batch(a, x, held, n, y, sm_count, fit, fault, st);
     FewArgs args = {};
     args.a = a;
     args.x.n = n, args.x.n_cols = a.n_cols;

@@ -30,6 +30,7 @@ constexpr unsigned kStages = 5;
 constexpr unsigned kX = 16384, kScalesA = kX + kRows * 128, kScalesX = kScalesA + 512, kStageBytes = kScalesX + 512;
 static_assert(kStageBytes % 1024 == 0, "blocks on 1024-byte boundaries");
 constexpr unsigned kThreads = 320;
+constexpr size_t kSharedBytes = kStages * kStageBytes + 1024;
 // A team that comes to a stage has waited for the step that is a round of teams and a round of stages behind it. With more teams than stages that would say nothing of
 // the stage's last step but one, and the wait for the last one, which is for a parity, could take one for the other.
 constexpr unsigned kTeams = 4;
@@ -225,30 +226,33 @@ template <class X, class Y> __global__ void __launch_bounds__(kThreads, 2) k_blo
 // Two CTAs share an SM, and its tensor memory. The driver, when asked, counts one for kernels that take any, so it is asked about this one, which is never launched.
 __global__ void __launch_bounds__(kThreads, 2) k_without_tensor_memory() {}
 
-template <class X, class Y> cudaError_t batch(const CUtensorMap &map_a, BatchArgs &p, int sm_count, cudaStream_t st)
+template <class X, class Y> cudaError_t batch(const CUtensorMap &map_a, const BatchArgs &p, cudaStream_t st)
 {
     auto *kernel = k_block8_batch<X, Y>;
-    const size_t smem = kStages * kStageBytes + 1024;
-    static SharedAllowance allowance, as_much;
-    static ClusterRoom room;
-    unsigned fit[9];
-    cudaError_t e = allowance.need((const void *)kernel, (int)smem);
-    if (e == cudaSuccess) e = as_much.need((const void *)k_without_tensor_memory, (int)smem);
-    if (e == cudaSuccess) e = room.most((const void *)k_without_tensor_memory, kThreads, smem, fit);
+    static SharedAllowance allowance;
+    const cudaError_t e = allowance.need((const void *)kernel, (int)kSharedBytes);
     if (e != cudaSuccess) return e;
-    p.n_split = host::block8_batch_split(p.a.n_block_rows, p.a.longest, sm_count, fit);
-    return launch_pdl_cluster(kernel, p.n_split, dim3(p.a.n_block_rows * p.n_split), dim3(kThreads), smem, st, map_a, p);
+    return launch_pdl_cluster(kernel, p.n_split, dim3(p.a.n_block_rows * p.n_split), dim3(kThreads), kSharedBytes, st, map_a, p);
 }
-template <class Y> cudaError_t batch_of(int dtype, const CUtensorMap &map_a, BatchArgs &p, int sm_count, cudaStream_t st)
+template <class Y> cudaError_t batch_of(int dtype, const CUtensorMap &map_a, const BatchArgs &p, cudaStream_t st)
 {
-    if (dtype < 0) return batch<Held, Y>(map_a, p, sm_count, st);
-    if (dtype == ASP_F32) return batch<float, Y>(map_a, p, sm_count, st);
-    if (dtype == ASP_F16) return batch<__half, Y>(map_a, p, sm_count, st);
-    return batch<__nv_bfloat16, Y>(map_a, p, sm_count, st);
+    if (dtype < 0) return batch<Held, Y>(map_a, p, st);
+    if (dtype == ASP_F32) return batch<float, Y>(map_a, p, st);
+    if (dtype == ASP_F16) return batch<__half, Y>(map_a, p, st);
+    return batch<__nv_bfloat16, Y>(map_a, p, st);
 }
 } // namespace
 
-cudaError_t launch_block8_batch(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, unsigned *fault, cudaStream_t st)
+cudaError_t block8_batch_room(unsigned fit[9])
+{
+    static SharedAllowance allowance;
+    static ClusterRoom room;
+    const void *kernel = (const void *)k_without_tensor_memory;
+    const cudaError_t e = allowance.need(kernel, (int)kSharedBytes);
+    return e == cudaSuccess ? room.most(kernel, kThreads, kSharedBytes, fit) : e;
+}
+
+cudaError_t launch_block8_batch(const Block8Dev &a, const Dense *x, const Rows8Dev *held, unsigned n, const Dense &y, int sm_count, const unsigned *fit, unsigned *fault, cudaStream_t st)
 {
     BatchArgs p = {};
     p.a = a, p.y = y.p, p.ldy = y.ld, p.fault = fault;
@@ -256,12 +260,13 @@ cudaError_t launch_block8_batch(const Block8Dev &a, const Dense *x, const Rows8D
     if (held) p.x.held = *held;
     else p.x.p = x->p, p.x.ld = x->ld;
     p.teams = n <= 8 ? 4 : 2;
+    p.n_split = host::block8_batch_split(a.n_block_rows, a.longest, sm_count, fit);
     CUtensorMap map_a;
     const cudaError_t e = byte_map(&map_a, a.values, 128, (uint64_t)(a.n_blocks ? a.n_blocks : 1) * 128, 128, 128);
     if (e != cudaSuccess) return e;
     const int from = held ? -1 : x->dtype;
-    if (y.dtype == ASP_F32) return batch_of<float>(from, map_a, p, sm_count, st);
-    if (y.dtype == ASP_F16) return batch_of<__half>(from, map_a, p, sm_count, st);
-    return batch_of<__nv_bfloat16>(from, map_a, p, sm_count, st);
+    if (y.dtype == ASP_F32) return batch_of<float>(from, map_a, p, st);
+    if (y.dtype == ASP_F16) return batch_of<__half>(from, map_a, p, st);
+    return batch_of<__nv_bfloat16>(from, map_a, p, st);
 }
 } // namespace asp

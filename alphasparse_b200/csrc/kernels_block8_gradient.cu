@@ -26,7 +26,7 @@ using namespace block8;
 // What bounds it is shared memory, 128 bytes a clock and SM: for 64 rows t, x of a block column passes it four times (8 KB in, 8 out, unfolded 16 in and
 // with each product 16 out), dy of a block row twice and more. Two blocks of a column share x: 56 KB a block instead of 80 for one alone, 448 clocks
 // where the products take 256. (Four would be 384, but leave no room for a second D: measured the same, with the rows below in one sum.) A quarter of
-// 4096 x 4096 by 4096 rows in bf16: 44.7 us, 770 TFLOP/s; of 8192 x 4096 by 8192: 165 us, 830 TFLOP/s, and 197 over and over, at the power limit.
+// 4096 x 4096 by 4096 rows in bf16: 42.3 us, 815 TFLOP/s; of 8192 x 4096 by 8192: 161 us, 855 TFLOP/s, and 197 over and over, at the power limit.
 //
 // Tensor cores cut off what they add up to, which over 8192 rows in one sum showed as 6.5e-6 of the result, where sums that are rounded have 6e-7. So D takes
 // 1280 rows in bf16 (8e-7), 768 in fp16, whose products have more bits (8e-7; 1.4e-6 with 1280), then another one the next, while the first is added,
@@ -46,7 +46,7 @@ constexpr unsigned kUnfolded = 3, kUnfoldedBytes = 2 * kTile; // x in 16 bits: 6
 constexpr unsigned kThreads = 896;
 constexpr size_t kSharedBytes = kRoom * kBlockBytes + kUnfolded * kUnfoldedBytes + kHeld * kHeldBytes + 1024;
 // Rows of dy that are not all on 16-byte boundaries cannot be copied by tiles. The warps that unfold x bring them, one of their steps ahead, in the aligned
-// pieces of 16 bytes that they lie in, and shift them to where they belong: 4001 rows, a quarter of 4001 x 4003, take 133 us (450 element by
+// pieces of 16 bytes that they lie in, and shift them to where they belong: 4001 rows, a quarter of 4001 x 4003, take 122 us (450 element by
 // element) where 4096 rows of 4096 x 4096 take 42 by tiles. They then take a part of dy's room, and groups are single blocks.
 constexpr unsigned kPitch = 272, kRawBytes = kRows * kPitch, kShiftedStages = 3; // 17 pieces a row
 static_assert(kShiftedStages * kBlockBytes + 4 * kRawBytes <= kRoom * kBlockBytes, "two steps of each group of warps beside the stages");

@@ -32,9 +32,9 @@ using namespace block8;
 // some columns each.
 //
 // What bounds it is shared memory, 128 bytes a clock and SM: a step writes 40 KB to it and the products read 40 KB, 640 clocks where the products alone
-// take 384. Rows, columns and rows of X, share of blocks stored: 8192, 8192, 8192, half: 247 us, 2.23 PFLOP/s in a burst; called over and over the chip comes to its
-// power limit and 1.28 GHz, and it takes 303. 4096, 4096, 2048, a quarter: 18 us, 0.95 PFLOP/s (512 tiles over 148 SMs, the last wave half empty,
-// and each CTA's first copies and last stores).
+// take 384. Rows, columns and rows of X, share of blocks stored: 8192, 8192, 8192, half: 256 us, 2.15 PFLOP/s in a burst; called over and over the chip comes to its
+// power limit and 1.28 GHz, and it takes 303. 4096, 4096, 2048, a quarter: 15.6 us, 1.10 PFLOP/s (352 tiles of unequal length over 148 SMs: 16,000 clocks of steps in
+// the longest CTA, 12,200 on average, and each CTA's first copies and last stores).
 //
 // A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 17 store.
 constexpr unsigned kMostRows = host::kBlock8ProductRows;
@@ -69,7 +69,7 @@ struct Shared
 };
 
 // The steps of a CTA, in order: the blocks of its tiles. Tiles are in the order of their block rows, longest first, and handed out to the CTAs forwards and backwards in
-// turn, so that who has a long one gets a short one next (a quarter of 4096 x 4096 by 2048 rows: 17.8 us, 19.1 with block rows side by side and always
+// turn, so that who has a long one gets a short one next (a quarter of 4096 x 4096 by 2048 rows, where eight warps stored: 17.8 us, 19.1 with block rows side by side and always
 // forwards). What a CTA has to know of a tile is asked for a tile ahead (17.8 to 17.0 us).
 // Where X is larger than a part of L2 it is gone through in parts of `wide` tiles, each with all block rows.
 struct Steps

@@ -37,8 +37,8 @@ int main()
             const unsigned b = block8_batch_split(rows, longest, sms, fit2);
             CHECK(b >= 1 && b <= s && (b == s || rows * b <= (unsigned)sms));
             batch.insert(b);
-            for (unsigned n : {1u, 8u, 9u, 32u}) which.insert(block8_batch(rows, longest, n, false, sms));
-            CHECK(!block8_batch(rows, longest, 32, true, sms) || block8_batch(rows, longest, 32, false, sms));
+            for (unsigned n : {1u, 8u, 9u, 32u}) which.insert(block8_batch(rows, longest, n, false, sms, fit2));
+            CHECK(!block8_batch(rows, longest, 32, true, sms, fit2) || (block8_batch(rows, longest, 32, false, sms, fit2) && longest <= b * kBlock8Sum));
             for (unsigned n = 33; n < 100000; n = n * 3 / 2)
             {
                 const Block8ProductPlan p = block8_product_plan(rows, (unsigned)(0.7 * rows * longest), longest, n, sms, fit1);
