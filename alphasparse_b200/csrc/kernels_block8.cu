@@ -166,18 +166,21 @@ __global__ void __launch_bounds__(256) k_block8_get(const uint8_t *values, const
 // A block row is shared by a cluster of CTAs, a contiguous piece of its blocks each, so that all SMs read; the cluster adds up the pieces in
 // order in one another's shared memory: no atomics, no room, the same bits every time.
 //
+// A form for each 8 rows: 19 rows, 60 % of 4001 x 2047, 7.5 us, 7.9 by the one for 32.
+//
 // X is converted for 4 / NT blocks at a time, which is a row's block to each eight lanes, and asked for while the stage before the one before is
 // multiplied: a stage's X is in shared memory, the next one's in registers.
 //
 // One row of bf16, half of 1024 x 1024: 3.1 us, of which the blocks are the least: a launch, X on its way and converted, the products, the cluster's sum. 4096 x 4096, all
-// of it: 6.0 us, 2.8 TB/s.
+// of it: 6.0 us, 2.8 TB/s, where the matrix is in L2, 7.7 where it is not.
 constexpr int kFewPitch = 272; // bytes a row and block: 16-byte reads of 8 lanes in 2 rows meet no conflict
-template <int NT> constexpr int kFewAhead = NT == 4 ? 4 : 5; // blocks on their way: two CTAs' 128 or 160 KB an SM, with room for X
+template <int NT> constexpr int kFewAhead = NT >= 3 ? 4 : 5; // blocks on their way: two CTAs' 128 or 160 KB an SM, with room for X
 template <int NT> struct FewShared
 {
     uint4 a[kFewAhead<NT>][4][256];
-    uint8_t x[2][4 / NT][8 * NT][kFewPitch];
-    float2 factor[2][4 / NT][8 * NT];
+    static constexpr unsigned per = 4 / NT; // blocks a stage
+    uint8_t x[2][per][8 * NT][kFewPitch];
+    float2 factor[2][per][8 * NT];
     float part[8 * NT][132];
 };
 
@@ -239,7 +242,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     const unsigned j0 = lo + (unsigned)((uint64_t)len * piece / split), j1 = lo + (unsigned)((uint64_t)len * (piece + 1) / split);
     const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
 
-    constexpr unsigned per = 4 / NT; // blocks a stage
+    constexpr unsigned per = FewShared<NT>::per;
     const uint8_t *mine = args.a.values + (warp * 16 + g) * 128 + 16 * q;
     const auto load = [&](unsigned j) { // (a group of copies for each block, empty ones behind the last)
         if (j < j1)
@@ -285,7 +288,7 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     if (threadIdx.x == 0 && j0 < j1)
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(args.a.values + (uint64_t)j0 * 16384), "r"(min(j1 - j0, 8u) * 16384) : "memory");
     for (unsigned i = threadIdx.x; i < sizeof(sh.x) / 16; i += 256) reinterpret_cast<uint4 *>(sh.x)[i] = make_uint4(0, 0, 0, 0);
-    for (unsigned i = threadIdx.x; i < 2 * 32; i += 256) (&sh.factor[0][0][0])[i] = make_float2(1.f, 1.f);
+    for (unsigned i = threadIdx.x; i < 2 * per * 8 * NT; i += 256) (&sh.factor[0][0][0])[i] = make_float2(1.f, 1.f);
     grid_wait();
     grid_release();
 #pragma unroll
@@ -294,14 +297,14 @@ template <int NT, class X, class Y> __global__ void __launch_bounds__(256, 2) k_
     Fetched<X> got = {};
     unsigned block_scale = 127;
     const auto ask = [&](unsigned j) { // of the stage that begins with block j
-        if (j + slot >= j1 || t >= tokens) return;
+        if (j + slot >= j1 || slot >= per || t >= tokens) return; // (24 rows leave 8 tasks over)
         got.ask(args.x, t, args.a.col[j + slot], lane8);
         block_scale = args.a.scales[j + slot];
     };
     const auto convert = [&](unsigned j) {
         const unsigned at = (j - j0) / per % 2;
-        const bool there = j + slot < j1 && t < tokens;
-        const unsigned both = put(got, sh.x[at][slot][t], lane8, there) + block_scale, half = both / 2; // exponents + 127 each
+        const bool there = j + slot < j1 && slot < per && t < tokens;
+        const unsigned both = put(got, sh.x[at][slot % per][t], lane8, there) + block_scale, half = both / 2; // exponents + 127 each
         if (there && lane8 == 0) sh.factor[at][slot][t] = make_float2(power(half), power(both - half));
     };
     ask(j0);
@@ -363,6 +366,7 @@ template <class X, class Y> cudaError_t few_by_rows(FewArgs &args, cudaStream_t 
 {
     if (args.x.n <= 8) return few<1, X, Y>(args, st);
     if (args.x.n <= 16) return few<2, X, Y>(args, st);
+    if (args.x.n <= 24) return few<3, X, Y>(args, st);
     return few<4, X, Y>(args, st);
 }
 } // namespace

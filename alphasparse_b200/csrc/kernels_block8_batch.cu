@@ -23,8 +23,9 @@ using namespace block8;
 //
 // A block row is shared by a cluster of CTAs, a contiguous piece of its blocks each; the cluster adds up the pieces in order in one another's shared memory.
 //
-// 8192 x 8192, all of it, bf16: 1 row 10.0 us (6.9 TB/s, some of it from L2), 16 rows 13.0, 32 rows 17.7; X in 8 bits already: 9.9, 11.3, 12.9. With products by mma.sync, which
-// then bound it, 13.6, 20.2 and 31.2.
+// 8192 x 8192, all of it, bf16: 1 row 10.0 us (6.9 TB/s, much of it from L2), 16 rows 13.0, 32 rows 17.7; X in 8 bits already: 9.9, 11.3, 12.9. With products by mma.sync, which
+// then bound it, 13.6, 20.2 and 31.2. Three matrices in turn, so that all comes from memory: 14.5 (4.8 TB/s; 10.3 for the bytes, the rest first copies, the cluster's
+// sum and the next launch), 17.2, 20.2; by mma.sync 15.4, 22.1, 32.7.
 constexpr unsigned kRows = 32;
 constexpr unsigned kStages = 5;
 constexpr unsigned kX = 16384, kScalesA = kX + kRows * 128, kScalesX = kScalesA + 512, kStageBytes = kScalesX + 512;

@@ -268,6 +268,24 @@ def test_apply(asp_ctx, n, n_rows, n_cols, density, transposed):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n_rows,n_cols,density", [(1000, 130, 0.5), (900, 2100, 0.3), (4001, 600, 0.9)])
+@pytest.mark.parametrize("n", [7, 16, 18, 23, 24, 25])
+def test_apply_to_short_block_rows(asp_ctx, n, n_rows, n_cols, density, dtype):
+    m, a = matrix(asp_ctx, n_rows + n, n_rows, n_cols, density, transposed=False, empty_row=1)
+    x, held = rows(n, n, n_cols, dtype, 1), Rows8(asp_ctx, n, n_cols)
+    y, other = (torch.full((n + 1, n_rows), 7.0, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    m.apply(x.data_ptr(), n, dtype, y.data_ptr(), "f32", n_cols + 1)
+    held.quantize(x.data_ptr(), n, dtype, n_cols + 1)
+    m.product(held, other.data_ptr(), "f32")
+    asp_ctx.synchronize()
+    assert_sums(y[:n], ref.rows_in_8_bits(x), a, "f32", f"apply {n} {dtype}")
+    assert (y[n] == 7.0).all() and torch.equal(y, other)
+    m.close()
+    held.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n_rows,n_cols,density,pad,offset", [(300, 9000, 0.9, 0, 0), (2500, 3500, 0.8, 1, 0), (5000, 2600, 1.0, 0, 3), (130, 8195, 0.6, 5, 0)])
 @pytest.mark.parametrize("n", [1, 4, 8, 9, 16, 17, 20, 31, 32])
 def test_apply_to_long_block_rows(asp_ctx, n, n_rows, n_cols, density, pad, offset, dtype):
