@@ -772,6 +772,50 @@ def test_same_bits_every_time_and_on_two_streams_at_once(asp_ctx):
     other.close()
 
 
+def test_calls_of_all_kinds_in_any_order_on_two_streams(asp_ctx):
+    """Kernels that share SMs, shared memory and tensor memory with others: the same bits as when each runs alone."""
+    other, calls, kept = capi.Context(0), [], []
+    for ctx in (asp_ctx, other):
+        for n_rows, n_cols, density in ((260, 6000, 0.9), (4096, 2048, 1.0), (1000, 1000, 0.5)):
+            m = Block8(ctx, n_rows, n_cols, *pattern(n_rows, n_rows, n_cols, density))
+            values = torch.randn(m.n_blocks, 128, 128, generator=gen(n_rows), device="cuda")
+            torch.cuda.synchronize()
+            m.set_values(values.data_ptr(), "f32")
+            ctx.synchronize()
+            for n, dtype in ((1, "bf16"), (7, "f16"), (13, "bf16"), (20, "f32"), (32, "f16"), (300, "f32"), (500, "bf16")):
+                x, y, held = rows(n, n, n_cols, dtype), torch.empty(n, n_rows, device="cuda"), Rows8(ctx, n, n_cols)
+                torch.cuda.synchronize()
+                held.quantize(x.data_ptr(), n, dtype)
+                ctx.synchronize()
+                kept.append((m, x, held))
+                if n <= 32:
+                    calls.append((lambda m=m, x=x, n=n, dtype=dtype, y=y: m.apply(x.data_ptr(), n, dtype, y.data_ptr(), "f32"), y))
+                else:
+                    calls.append((lambda m=m, held=held, y=y: m.product(held, y.data_ptr(), "f32"), y))
+                if dtype == "bf16":
+                    dy, da = rows(n + 1, n, n_rows, dtype), torch.empty(m.n_blocks, 128, 128, device="cuda")
+                    kept.append(dy)
+                    calls.append((lambda m=m, held=held, dy=dy, da=da: m.gradient(held, dy.data_ptr(), "bf16", da.data_ptr()), da))
+    torch.cuda.synchronize()
+    alone = []
+    for call, out in calls:
+        call()
+        asp_ctx.synchronize()
+        other.synchronize()
+        alone.append(out.clone())
+    rng = np.random.default_rng(1)
+    for _ in range(5):
+        for _, out in calls:
+            out.fill_(7.0)
+        torch.cuda.synchronize()
+        for i in np.concatenate([rng.permutation(len(calls)) for _ in range(3)]):
+            calls[i][0]()
+        asp_ctx.synchronize()
+        other.synchronize()
+        assert all(torch.equal(out, want) for (_, out), want in zip(calls, alone))
+    other.close()
+
+
 def test_more_than_2_to_the_31_bytes_of_rows(asp_ctx):
     """Rows behind byte 2^32 of X and of Y; values behind byte 2^32 of A would need 2^18 blocks and are held to 64-bit products in the code."""
     n, c = 600_000, 8192
