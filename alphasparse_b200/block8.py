@@ -6,6 +6,7 @@ Everything takes device pointers (ints) and runs on the stream of its Context, l
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -54,6 +55,27 @@ def _bind_apply(ctx_handle, handle):
     return native(C.cast(_lib().asp_block8_apply, C.c_void_p).value, C.addressof(ctx_handle), C.addressof(handle))
 
 
+def _bind(name, ctx_handle, handle):
+    """Another call of (context, handle, ...) with the two given: without ctypes where that binding has been built, and through it. Both handles are read at
+    every call; the caller keeps them alive."""
+    fn = getattr(_lib(), name)
+    plain = functools.partial(fn, ctx_handle, handle)
+    try:
+        native = capi._native().Bound
+    except (ImportError, AttributeError):
+        return plain, plain
+    return native(name, C.cast(fn, C.c_void_p).value, C.addressof(ctx_handle), C.addressof(handle)), plain
+
+
+def _run(call, *args) -> None:
+    try:
+        status = call[0](*args)
+    except TypeError:  # whatever else ctypes takes for a pointer
+        status = call[1](*args)
+    if status:
+        capi.check(status)
+
+
 class Rows8:
     """asp_rows8: up to max_rows rows of n_cols columns in 8 bits, a scale for each row and 128 columns."""
 
@@ -61,6 +83,8 @@ class Rows8:
         self._h = C.c_void_p()
         self.ctx, self.max_rows, self.n_cols = ctx, max_rows, n_cols
         capi.check(_lib().asp_rows8_create(ctx.handle, max_rows, n_cols, C.byref(self._h)))
+        self._ctx_handle = ctx.handle  # kept alive: calls may have no more than its address and that of our own
+        self._quantize, self._restore = (_bind(name, self._ctx_handle, self._h) for name in ("asp_rows8_quantize", "asp_rows8_restore"))
 
     def __len__(self) -> int:
         """Rows held."""
@@ -68,16 +92,16 @@ class Rows8:
 
     def quantize(self, x: int, n: int, dtype: str, ld: int = 0) -> None:
         """n rows at x to 8 bits."""
-        capi.check(_lib().asp_rows8_quantize(self.ctx.handle, self._h, x, TYPES[dtype], n, ld))
+        _run(self._quantize, x, TYPES[dtype], n, ld)
 
     def restore(self, out: int, dtype: str, ld: int = 0) -> None:
         """What the rows held stand for."""
-        capi.check(_lib().asp_rows8_restore(self.ctx.handle, self._h, out, TYPES[dtype], ld))
+        _run(self._restore, out, TYPES[dtype], ld)
 
     def close(self):
         if self._h:
             _lib().asp_rows8_destroy(self._h)
-            self._h = C.c_void_p()
+            self._h.value = None  # (in place: its address is held)
 
     def __del__(self):
         try:
@@ -113,8 +137,10 @@ class Block8:
 
     def _take(self, ctx, h, n_rows, n_cols):
         self._h, self.ctx, self.n_rows, self.n_cols = h, ctx, n_rows, n_cols
-        self._ctx_handle = ctx.handle  # kept alive: _call may have no more than its address and that of our own
+        self._ctx_handle = ctx.handle  # kept alive: calls may have no more than its address and that of our own
         self._apply = _bind_apply(self._ctx_handle, h)
+        self._set, self._get, self._product, self._gradient = (
+            _bind(f"asp_block8_{name}", self._ctx_handle, h) for name in ("set_values", "get_values", "product", "gradient"))
         self.n_blocks = int(_lib().asp_block8_blocks(h))
 
     def pattern(self):
@@ -128,11 +154,11 @@ class Block8:
 
     def set_values(self, values: int, dtype: str) -> None:
         """New values of all stored blocks, [n_blocks, 128, 128]."""
-        capi.check(_lib().asp_block8_set_values(self.ctx.handle, self._h, values, TYPES[dtype]))
+        _run(self._set, values, TYPES[dtype])
 
     def get_values(self, values: int) -> None:
         """What the stored blocks stand for, [n_blocks, 128, 128] in 32 bits."""
-        capi.check(_lib().asp_block8_get_values(self.ctx.handle, self._h, values))
+        _run(self._get, values)
 
     def apply(self, x: int, n: int, x_dtype: str, y: int, y_dtype: str, ldx: int = 0, ldy: int = 0, transposed: bool = False) -> None:
         """y = A x (transposed: A^T x) for n <= 32 rows x in 16 or 32 bits, converted to 8 bits on the way."""
@@ -146,11 +172,11 @@ class Block8:
 
     def product(self, x: Rows8, y: int, dtype: str, ld: int = 0, transposed: bool = False) -> None:
         """y = A x (transposed: A^T x) for the rows that x holds."""
-        capi.check(_lib().asp_block8_product(self.ctx.handle, self._h, transposed, x._h, y, TYPES[dtype], ld))
+        _run(self._product, transposed, x._h.value or 0, y, TYPES[dtype], ld)
 
     def gradient(self, x: Rows8, dy: int, dtype: str, out: int, ld: int = 0, accumulate: bool = False) -> None:
         """The gradient by the stored blocks, [n_blocks, 128, 128] in 32 bits, from dy and the rows x kept in 8 bits."""
-        capi.check(_lib().asp_block8_gradient(self.ctx.handle, self._h, x._h, dy, TYPES[dtype], ld, out, int(accumulate)))
+        _run(self._gradient, x._h.value or 0, dy, TYPES[dtype], ld, out, int(accumulate))
 
     def close(self):
         if self._h:

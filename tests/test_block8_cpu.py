@@ -150,3 +150,47 @@ def test_apply_with_and_without_the_binding(monkeypatch):
         with pytest.raises(C.ArgumentError):
             m.apply(1.5, 1, "f32", 16, "f32")
         monkeypatch.setattr(capi, "_native", none)
+
+
+CALLS = {
+    "asp_rows8_quantize": (C.c_void_p, C.c_int, C.c_uint64, C.c_uint64),
+    "asp_rows8_restore": (C.c_void_p, C.c_int, C.c_uint64),
+    "asp_block8_set_values": (C.c_void_p, C.c_int),
+    "asp_block8_get_values": (C.c_void_p,),
+    "asp_block8_product": (C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_uint64),
+    "asp_block8_gradient": (C.c_void_p, C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_int),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_calls_without_ctypes_hand_on_what_they_are_given(name):
+    seen = []
+    fn = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p, *CALLS[name])(lambda *args: seen.append(args) or 3)
+    ctx, handle = C.c_void_p(0x1230), C.c_void_p(0x4560)
+    call = capi._native().Bound(name, C.cast(fn, C.c_void_p).value, C.addressof(ctx), C.addressof(handle))
+    args = [2**63 + 16 * i if t in (C.c_void_p, C.c_uint64) else i + 1 for i, t in enumerate(CALLS[name])]
+    assert call(*args) == 3 and list(seen[-1]) == [0x1230, 0x4560] + args
+    handle.value = ctx.value = None  # both are read at the call
+    assert call(*args) == 3 and list(seen[-1]) == [None, None] + args
+    for bad in ([None] + args[1:], args[1:], args + [0], args[:-1] + [1.5]):
+        with pytest.raises(TypeError):
+            call(*bad)
+    with pytest.raises(ValueError):
+        capi._native().Bound("asp_" + name, 0, 0, 0)
+
+
+def test_closed_handles_and_other_pointers(monkeypatch):
+    def none():
+        raise ImportError
+
+    for _ in range(2):
+        h, ctx = C.c_void_p(), C.c_void_p()
+        quantize, product = block8._bind("asp_rows8_quantize", ctx, h), block8._bind("asp_block8_product", ctx, h)
+        for x in (16, None, C.c_void_p(16)):
+            for call, args in ((quantize, (x, 4, 1, 0)), (product, (False, 0, x, 4, 0))):
+                with pytest.raises(capi.AspError) as e:
+                    block8._run(call, *args)
+                assert e.value.status == 1
+        with pytest.raises(C.ArgumentError):
+            block8._run(quantize, 1.5, 4, 1, 0)
+        monkeypatch.setattr(capi, "_native", none)
