@@ -19,7 +19,8 @@ unsigned largest(unsigned n_block_rows, unsigned longest, unsigned ctas, const u
 }
 } // namespace
 
-unsigned block8_few_split(unsigned n_block_rows, unsigned longest, const unsigned *fit) { return largest(n_block_rows, longest, ~0u, fit); }
+// What a CTA converts and multiplies at once is not shared out: a cluster's start and sum cost more (8 rows of 12000 x 384 4.0 us instead of 5.1, 14 rows of 4096 x 256 4.0 instead of 4.8).
+unsigned block8_few_split(unsigned n_block_rows, unsigned longest, unsigned per, const unsigned *fit) { return longest <= per ? 1 : largest(n_block_rows, longest, ~0u, fit); }
 
 // One CTA an SM where its blocks are few (16 rows of 4096 x 4096: 8 blocks to each of 128 CTAs 7.5 us, 4 to each of 256 8.2), two where they are many (one row of 8192 x 8192:
 // 32 to 128 11.9 us, 16 to 256 9.9).

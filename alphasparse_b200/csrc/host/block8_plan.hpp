@@ -15,7 +15,7 @@ constexpr unsigned kBlock8Sum = 16;
 // Products with up to 32 rows: by the kernel for few rows or for a batch (k_block8_few, k_block8_batch)?
 bool block8_batch(unsigned n_block_rows, unsigned longest, unsigned n, bool wide, int sm_count, const unsigned *fit);
 // and CTAs that share the blocks of a block row
-unsigned block8_few_split(unsigned n_block_rows, unsigned longest, const unsigned *fit);
+unsigned block8_few_split(unsigned n_block_rows, unsigned longest, unsigned per, const unsigned *fit); // per: blocks whose rows of X are converted at once
 unsigned block8_batch_split(unsigned n_block_rows, unsigned longest, int sm_count, const unsigned *fit);
 
 // Products with many rows (k_block8_product): rows of X a tile (64, 128, 192), and CTAs that share the blocks of a tile (1 to 8).

@@ -359,7 +359,7 @@ template <int NT, class X, class Y> cudaError_t few(FewArgs &args, cudaStream_t 
     cudaError_t e = allowance.need((const void *)kernel, (int)smem);
     if (e == cudaSuccess) e = room.most((const void *)kernel, 256, smem, fit);
     if (e != cudaSuccess) return e;
-    args.n_split = host::block8_few_split(args.a.n_block_rows, args.a.longest, fit);
+    args.n_split = host::block8_few_split(args.a.n_block_rows, args.a.longest, FewShared<NT>::per, fit);
     return launch_pdl_cluster(kernel, args.n_split, dim3(args.a.n_block_rows * args.n_split), dim3(256), smem, st, args);
 }
 template <class X, class Y> cudaError_t few_by_rows(FewArgs &args, cudaStream_t st)

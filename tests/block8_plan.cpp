@@ -31,7 +31,8 @@ int main()
     for (unsigned rows = 1; rows < 70000; rows = rows < 160 ? rows + 1 : rows * 3 / 2)
         for (unsigned longest = 0; longest < 3000; longest = longest * 2 + 1)
         {
-            const unsigned s = block8_few_split(rows, longest, fit2);
+            const unsigned s = block8_few_split(rows, longest, 1, fit2);
+            for (unsigned per : {2u, 4u}) CHECK(block8_few_split(rows, longest, per, fit2) == (longest <= per ? 1 : s));
             CHECK(s >= 1 && s <= 8 && (s == 1 || s <= longest) && (s == 1 || rows <= fit2[s]));
             few.insert(s);
             const unsigned b = block8_batch_split(rows, longest, sms, fit2);
