@@ -26,7 +26,7 @@ using namespace block8;
 // What bounds it is shared memory, 128 bytes a clock and SM: for 64 rows t, x of a block column passes it four times (8 KB in, 8 out, unfolded 16 in and
 // with each product 16 out), dy of a block row twice and more. Two blocks of a column share x: 56 KB a block instead of 80 for one alone, 448 clocks
 // where the products take 256. (Four would be 384, but leave no room for a second D: measured the same, with the rows below in one sum.) A quarter of
-// 4096 x 4096 by 4096 rows in bf16: 42.3 us, 815 TFLOP/s; of 8192 x 4096 by 8192: 161 us, 855 TFLOP/s, and 197 over and over, at the power limit.
+// 4096 x 4096 by 4096 rows in bf16: 42.3 us, 815 TFLOP/s; of 8192 x 4096 by 8192: 161 us, 855 TFLOP/s, and 184 over and over, at the power limit.
 //
 // Tensor cores cut off what they add up to, which over 8192 rows in one sum showed as 6.5e-6 of the result, where sums that are rounded have 6e-7. So D takes
 // 1280 rows in bf16 (8e-7), 768 in fp16, whose products have more bits (8e-7; 1.4e-6 with 1280), then another one the next, while the first is added,

@@ -33,7 +33,7 @@ using namespace block8;
 //
 // What bounds it is shared memory, 128 bytes a clock and SM: a step writes 40 KB to it and the products read 40 KB, 640 clocks where the products alone
 // take 384. Rows, columns and rows of X, share of blocks stored: 8192, 8192, 8192, half: 256 us, 2.15 PFLOP/s in a burst; called over and over the chip comes to its
-// power limit and 1.28 GHz, and it takes 303. 4096, 4096, 2048, a quarter: 15.6 us, 1.10 PFLOP/s (352 tiles of unequal length over 148 SMs: 16,000 clocks of steps in
+// power limit and 1.28 GHz, and it takes 293. 4096, 4096, 2048, a quarter: 15.6 us, 1.10 PFLOP/s (352 tiles of unequal length over 148 SMs: 16,000 clocks of steps in
 // the longest CTA, 12,200 on average, and each CTA's first copies and last stores).
 //
 // A CTA per SM goes through tiles: warp 0 copies blocks, rows and their scales, warp 1 issues products, warps 2 to 17 store.
