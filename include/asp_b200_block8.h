@@ -46,7 +46,8 @@ asp_status asp_rows8_create(asp_ctx *ctx, uint64_t max_rows, uint64_t n_cols, as
 void asp_rows8_destroy(asp_rows8 *rows);
 /* X (n rows, ASP_F32 | ASP_F16 | ASP_BF16) to 8 bits; the handle then holds n rows. Rows behind them are left as they were. */
 asp_status asp_rows8_quantize(asp_ctx *ctx, asp_rows8 *rows, const void *d_x, int dtype, uint64_t n, uint64_t ld);
-/* What the rows held stand for, in any of the three types (rounded to nearest where the type cannot hold it). */
+/* What the rows held stand for, in any of the three types (rounded to nearest where the type cannot hold it: fp16 of 63488 and more has become 65536 in 8 bits, which
+ * is infinite in fp16). */
 asp_status asp_rows8_restore(asp_ctx *ctx, const asp_rows8 *rows, void *d_out, int dtype, uint64_t ld);
 /* rows held */
 uint64_t asp_rows8_count(const asp_rows8 *rows);
@@ -82,7 +83,8 @@ asp_status asp_block8_product(asp_ctx *ctx, const asp_block8 *m, int transposed,
 /* The gradient of a loss by the stored blocks, from the gradient dY by the rows of y = A x and the rows x kept in 8 bits:
  * dA[block (i, j)] = sum over the rows of dy[128 i + .] x[128 j + .]^T, 32 bits, in the order of asp_block8_set_values; zero outside the
  * matrix. dY: ASP_F16 | ASP_BF16, the type that x was converted from (ASP_ERR_UNSUPPORTED otherwise), so that the products' factors
- * are exact; as many rows as x holds. Rows of dY on 16-byte boundaries (d_dy, and ld a multiple of 8) are copied by tiles, others take up to three times as
+ * are exact; as many rows as x holds. What 8 bits have made of the type's largest numbers, 2^16 or 2^128, counts as that, although the type does not have it: rows
+ * with numbers above 57344 (fp16) or 1.75 * 2^127 (bf16) take some ten times as long as others. Rows of dY on 16-byte boundaries (d_dy, and ld a multiple of 8) are copied by tiles, others take up to three times as
  * long. accumulate != 0: added to d_out. d_out 16-byte aligned. Sums of at most 1280 rows are added up, rounded, in one order. */
 asp_status asp_block8_gradient(asp_ctx *ctx, const asp_block8 *m, const asp_rows8 *x, const void *d_dy, int dtype, uint64_t ld, float *d_out, int accumulate);
 

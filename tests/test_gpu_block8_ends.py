@@ -1,0 +1,80 @@
+"""GPU: block-sparse matrices in 8 bits (include/asp_b200_block8.h) at the ends of their types, and right after they are made. Tolerances as in test_gpu_block8.py."""
+import pytest
+import torch
+
+import block8_ref as ref
+from alphasparse_b200.block8 import Block8, Rows8
+from test_gpu_block8 import TYPES, assert_gradient, gen, pattern, rows
+
+pytestmark = pytest.mark.gpu
+
+# blocks of a block column, block columns, rows, elements between the rows of dy, by what takes them: a cluster that shares the rows, single blocks, twos, twos in
+# several sums, single blocks in several sums, rows of dy that begin anywhere
+WAYS = [(1, 3, 1000, 0), (1, 150, 200, 0), (2, 100, 150, 0), (2, 100, 2000, 0), (1, 150, 1500, 0), (2, 5, 300, 1), (3, 70, 150, 1), (3, 50, 70, 0)]
+
+
+def gradient(ctx, blocks, columns, x, dy, dtype, before=None):
+    """(the gradient by all blocks of a matrix of blocks x columns of them, added to `before` where it is given; the pattern)"""
+    n, n_rows, n_cols = x.shape[0], dy.shape[1], x.shape[1]
+    assert ref.blocks(n_rows) == blocks and ref.blocks(n_cols) == columns
+    p = pattern(1, n_rows, n_cols, 1.0)
+    m, held = Block8(ctx, n_rows, n_cols, *p), Rows8(ctx, n, n_cols)
+    out = torch.full((m.n_blocks, 128, 128), 7.0, device="cuda") if before is None else before.clone()
+    torch.cuda.synchronize()
+    held.quantize(x.data_ptr(), n, dtype)
+    m.gradient(held, dy.data_ptr(), dtype, out.data_ptr(), dy.stride(0) if n > 1 else 0, accumulate=before is not None)
+    ctx.synchronize()
+    m.close()
+    held.close()
+    return out, p
+
+
+def factors(blocks, columns, n, pad, dtype):
+    """x and dy of whole numbers of steps and not, dy with rows of zeros."""
+    x, dy = rows(n, n, 128 * columns - 5, dtype), rows(n + 1, n, (128 * blocks - 8), dtype, 8 if pad == 0 else pad)
+    dy[torch.rand(n, generator=gen(3), device="cuda") < 0.2] = 0.0
+    return x, dy
+
+
+def with_largest(x, dtype, share, seed=4):
+    """x, where `share` of the rows' blocks have some of the largest numbers of the type, which 8 bits round up to what the type does not have"""
+    g, (n, c) = gen(seed), x.shape
+    large = torch.tensor([63424.0, 63488.0, 65504.0] if dtype == "f16" else [247.0 * 2.0**120, 248.0 * 2.0**120, 255.0 * 2.0**120], device="cuda")
+    which = (torch.rand(n, ref.blocks(c), generator=g, device="cuda") < share).repeat_interleave(128, 1)[:, :c]
+    some = which & (torch.rand(n, c, generator=g, device="cuda") < 0.1)
+    v = large[torch.randint(0, 3, (n, c), generator=g, device="cuda")] * (torch.randint(0, 2, (n, c), generator=g, device="cuda") * 2 - 1)
+    return torch.where(some, v.to(TYPES[dtype]), x)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("blocks,columns,n,pad", WAYS)
+@pytest.mark.parametrize("share", [0.02, 1.0])
+def test_gradient_of_the_largest_numbers(asp_ctx, blocks, columns, n, pad, share, dtype):
+    """What 8 bits make of them, 2^16 and 2^128, is no number of the type. It still counts as what it is, and nothing where dy is zero."""
+    x, dy = factors(blocks, columns, n, pad, dtype)
+    x = with_largest(x, dtype, share)
+    if dtype == "bf16":
+        dy *= 2.0**-30  # (in place: its rows stay where they are)
+    want = ref.rows_in_8_bits(x)
+    assert (want.abs() > torch.finfo(TYPES[dtype]).max).any() and want.isfinite().all()
+    out, p = gradient(asp_ctx, blocks, columns, x, dy, dtype)
+    assert_gradient(out, dy, want, p)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("blocks,columns,n,pad", WAYS)
+def test_gradient_where_dy_is_not_finite(asp_ctx, blocks, columns, n, pad, dtype):
+    """Beside rows of the largest numbers and others: infinite and NaN as the formula has them, element by element."""
+    x, dy = factors(blocks, columns, n, pad, dtype)
+    x = torch.where(x == 0, torch.ones_like(x), with_largest(x, dtype, 0.02))
+    x[min(n - 1, 65), 7] = 0.0
+    dy *= 2.0**-30 if dtype == "bf16" else 1.0
+    dy[0, 5], dy[n // 2, 9], dy[min(n - 1, 65), 11], dy[n - 1, 1] = float("inf"), -float("inf"), float("inf"), float("nan")
+    out, p = gradient(asp_ctx, blocks, columns, x, dy, dtype)
+    xq, dyd = ref.rows_in_8_bits(x), dy.double()
+    want = ref.stored(p, dyd.T @ xq)
+    assert want.isnan().any() and want.isinf().any()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf()) and torch.equal(out[want.isinf()].double(), want[want.isinf()])
+    clean = torch.where(dyd.isfinite().all(0), dyd, 0.0)  # (columns of dy without any: rows of the blocks)
+    finite = ref.stored(p, (dyd.isfinite().all(0).double()[:, None] * torch.ones(1, x.shape[1], dtype=torch.float64, device="cuda")))
+    assert_gradient(torch.where(finite > 0, out, 0.0), clean, xq, p)
