@@ -97,11 +97,9 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
     const int sides = m->transposed ? 2 : 1;
     Piece values[2], scales[2], scale_rows[2], col[2], rows_of[2];
     std::vector<uint4> by_length[2];
+    // What is copied comes first and lies together: everything between the first array and the last is written by the copy.
     for (int s = 0; s < sides; s++)
     {
-        values[s] = take(n * kBlock8 * kBlock8);
-        scales[s] = take(n);
-        scale_rows[s] = take(n * 512);
         col[s] = take(n * 4);
         for (const uint32_t r : p.side[s].order) by_length[s].push_back({r, p.side[s].ptr[r], p.side[s].ptr[r + 1] - p.side[s].ptr[r], 0});
         rows_of[s] = take(by_length[s].size() * sizeof(uint4));
@@ -122,6 +120,12 @@ asp_status upload(asp_ctx *ctx, std::unique_ptr<asp_block8> &m)
             group[g].push_back(of);
         }
         groups[g] = take(group[g].size() * sizeof(asp::Block8Group));
+    }
+    for (int s = 0; s < sides; s++)
+    {
+        values[s] = take(n * kBlock8 * kBlock8);
+        scales[s] = take(n);
+        scale_rows[s] = take(n * 512);
     }
     ASP_ON_DEVICE(ctx);
     m->room.device = ctx->device;

@@ -68,7 +68,7 @@ class Stager
         void *with;
     };
     cudaError_t to_device(void *dev, const void *host, size_t bytes, cudaStream_t st, size_t piece, const Sent &sent);
-    // many arrays of one device block (ascending offsets): as few copies as the pieces make
+    // many arrays of one device block (ascending offsets): as few copies as the pieces make. What lies between them in the block is written over.
     cudaError_t to_device(void *dev, const std::vector<Segment> &segments, cudaStream_t st);
     cudaError_t to_device(void *dev, const Segment *segments, size_t count, cudaStream_t st, size_t piece = 0, const Sent *sent = nullptr);
     // complete on return

@@ -1,4 +1,5 @@
 """GPU: block-sparse matrices in 8 bits (include/asp_b200_block8.h) at the ends of their types, and right after they are made. Tolerances as in test_gpu_block8.py."""
+import numpy as np
 import pytest
 import torch
 
@@ -78,3 +79,28 @@ def test_gradient_where_dy_is_not_finite(asp_ctx, blocks, columns, n, pad, dtype
     clean = torch.where(dyd.isfinite().all(0), dyd, 0.0)  # (columns of dy without any: rows of the blocks)
     finite = ref.stored(p, (dyd.isfinite().all(0).double()[:, None] * torch.ones(1, x.shape[1], dtype=torch.float64, device="cuda")))
     assert_gradient(torch.where(finite > 0, out, 0.0), clean, xq, p)
+
+
+@pytest.mark.parametrize("rows_of_blocks,columns", [(3, 5), (40, 50)])
+def test_transposed_blocks_are_zero_until_they_have_values(asp_ctx, rows_of_blocks, columns):
+    """Whatever the context has copied to the device before: here a matrix without a zero among its values."""
+    from alphasparse_b200 import matrices
+    from alphasparse_b200.graph import Matrix
+
+    full, _ = matrices.from_row_lengths(np.full(2048, 2048), 2048, seed=2)
+    Block8.from_matrix(asp_ctx, Matrix.from_csr(full), transposed=True).close()
+    n_rows, n_cols = 128 * rows_of_blocks, 128 * columns
+    m = Block8(asp_ctx, n_rows, n_cols, *pattern(1, n_rows, n_cols, 1.0), transposed=True)
+    for transposed in (False, True):
+        c, r = (n_rows, n_cols) if transposed else (n_cols, n_rows)
+        for n in (1, 20, 100):
+            x, held = torch.ones(n, c, device="cuda"), Rows8(asp_ctx, n, c)
+            y, y1 = torch.full((n, r), 7.0, device="cuda"), torch.full((min(n, 32), r), 7.0, device="cuda")
+            torch.cuda.synchronize()
+            held.quantize(x.data_ptr(), n, "f32")
+            m.product(held, y.data_ptr(), "f32", transposed=transposed)
+            m.apply(x.data_ptr(), min(n, 32), "f32", y1.data_ptr(), "f32", transposed=transposed)
+            asp_ctx.synchronize()
+            assert (y == 0).all() and (y1 == 0).all(), (transposed, n)
+            held.close()
+    m.close()
