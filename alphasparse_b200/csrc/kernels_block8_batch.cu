@@ -153,7 +153,7 @@ template <class X, class Y> __global__ void __launch_bounds__(kThreads, 2) k_blo
             for (unsigned r = 0; r < 2; r++)
                 if (t - lane / 8 + 16 * r < p.x.n) scale[r] = got[r].eight(q[r], lane8); // (any row of the warp's)
             ask(j + p.teams);
-            all = __all_sync(~0u, tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up));
+            all = tc::warp_wait(&sh.empty[s], phase ^ 1, &sh.gave_up);
             if (!all) break;
             unsigned char *to = stages + s * kStageBytes;
 #pragma unroll
@@ -182,7 +182,7 @@ template <class X, class Y> __global__ void __launch_bounds__(kThreads, 2) k_blo
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) v[i] = 0.f;
-        if (j0 < j1 && __all_sync(~0u, all && tc::barrier_wait(&sh.done, 0, &sh.gave_up)))
+        if (j0 < j1 && all && tc::warp_wait(&sh.done, 0, &sh.gave_up))
         {
             tc::fence_after();
             tc::tensor_load16(tensor + first + (quarter * 32 << 16), v);

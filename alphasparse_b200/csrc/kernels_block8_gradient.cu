@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
             {
                 if (turn == mine)
                 {
-                    if (!tc::barrier_wait(&sh.held[x], x_phase, &sh.gave_up)) goto end;
+                    if (!tc::warp_wait(&sh.held[x], x_phase, &sh.gave_up)) goto end;
                     const unsigned char *from = bytes + x * kHeldBytes;
                     uint4 q[2];
                     unsigned scale[2];
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                     tc::fence_async_shared();
                     __syncwarp();
                     if (lane == 0) tc::barrier_arrive(&sh.read[x]);
-                    if (!tc::barrier_wait(&sh.used[h], h_phase ^ 1, &sh.gave_up)) goto end;
+                    if (!tc::warp_wait(&sh.used[h], h_phase ^ 1, &sh.gave_up)) goto end;
                     if (scale[0] == Unfold::largest || scale[1] == Unfold::largest) // (here, in front of all stores: inside words it takes 4 % of the time)
                     {
                         scale[0] -= scale[0] == Unfold::largest, scale[1] -= scale[1] == Unfold::largest;
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                         ask(next_u, next_i, parity ^ 1);
                         wait_for_all_groups_but<1>();
                         __syncwarp();
-                        if (!tc::barrier_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
+                        if (!tc::warp_wait(&sh.empty[s], phase ^ 1, &sh.gave_up)) goto end;
                         const int columns = (int)(p.n_rows - row * 128) - (int)(8 * j); // of the piece, that are in the matrix
 #pragma unroll
                         for (unsigned k = 0; k < 4; k++)
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
             const Places at = places<Unfold>(p, group, quarter, lane);
             for (unsigned i = step0; i < step1; i += Unfold::round)
             {
-                if (!tc::barrier_wait<64>(&sh.done[d], d_phase, &sh.gave_up)) goto end;
+                if (!tc::warp_wait<64>(&sh.done[d], d_phase, &sh.gave_up)) goto end;
                 tc::fence_after();
                 const bool last = i + Unfold::round >= step1 && p.split == 1;
                 for (unsigned c = mine; c < blocks * 128; c += 32)

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_product(const __grid_con
             bool all = true;
             while (at.j < at.end)
             {
-                all = tc::barrier_wait<64>(&sh.done[b], b_phase, &sh.gave_up);
+                all = tc::warp_wait<64>(&sh.done[b], b_phase, &sh.gave_up);
                 if (!all) break;
                 tc::fence_after();
 #pragma unroll

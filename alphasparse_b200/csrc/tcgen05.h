@@ -63,6 +63,11 @@ template <unsigned idle_ns = 0> __device__ __forceinline__ bool barrier_wait(uin
         }
     }
 }
+// For a warp that goes on as a whole: its lanes look one by one, and one may give up where another finds that it need not. True where all of them may go on.
+template <unsigned idle_ns = 0> __device__ __forceinline__ bool warp_wait(uint64_t *b, unsigned parity, volatile unsigned *gave_up)
+{
+    return __all_sync(~0u, barrier_wait<idle_ns>(b, parity, gave_up));
+}
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
