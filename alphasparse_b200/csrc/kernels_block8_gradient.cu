@@ -36,7 +36,7 @@ using namespace block8;
 //
 // 8 bits round up: the largest numbers of either 16-bit type become 256 times the largest scale, 2^16 or 2^128, which the type does not have. Rows with that scale
 // are unfolded to half of what they are, and a CTA that has met some adds the other half when it is done with its groups (add_halves). (A second pass of such steps through
-// the tensor cores has the issuing warp look at each step whether there are any, between two waits: 48.1 us instead of 44.5 for the quarter of 4096 x 4096, without any.)
+// the tensor cores has the issuing warp look at each step whether there are any, between two waits: 48.1 us instead of 45.4 for the quarter of 4096 x 4096, without any.)
 //
 // Warp 0 copies, warp 1 issues products, warps 4 to 11 add up and store, warps 12 to 19 and 20 to 27 unfold x, every second step each.
 constexpr unsigned kRows = host::kBlock8GradientRows; // t a step
@@ -87,6 +87,7 @@ struct Unfold16 // to fp16: in two factors, since the power may be below what fp
     static constexpr unsigned largest = 127 + 8;   // scale of what exceeds 57344: 256 times it is 2^16
     static __device__ __forceinline__ void words(uint4 q, unsigned scale, unsigned *out)
     {
+        scale = min(scale, largest - 1);
         const int k1 = max((int)scale, 127 - 14);
         const __half2 f1 = __float2half2_rn(power((unsigned)k1)), f2 = __float2half2_rn(power((unsigned)((int)scale - k1 + 127)));
         const unsigned in[4] = {q.x, q.y, q.z, q.w};
@@ -123,7 +124,7 @@ struct UnfoldB16
         }
         if (scale + 120 > 254)
 #pragma unroll
-            for (int i = 0; i < 8; i++) out[i] = product(out[i], ((scale + 120 - 254 + 127) << 7) * 0x10001u);
+            for (int i = 0; i < 8; i++) out[i] = product(out[i], ((min(scale, largest - 1) + 120 - 254 + 127) << 7) * 0x10001u);
         if (nan & 0x80808080u)
 #pragma unroll
             for (int i = 0; i < 16; i++)
@@ -178,7 +179,7 @@ __device__ __forceinline__ void store_columns(const Places &at, const float *v, 
 
 // The other half of the rows with the largest scale, to the result of a group, by the whole CTA: 32 such rows at a time come to shared memory as 32-bit numbers, and a
 // thread multiplies and adds for 4 columns of every 28th row of a block, in the order of the rows: the same bits every time.
-// A quarter of 4096 x 4096 by 4096 rows: 44.5 us without such rows (44.2 without the test for them), 65 with one, 89 with 64 in one block column, 1640 where all are in one.
+// A quarter of 4096 x 4096 by 4096 rows: 45.4 us without such rows (44.2 without the test for them and the votes of waits), 65 with one, 89 with 64 in one block column, 1640 where all are in one.
 constexpr unsigned kWarps = kThreads / 32, kHalvesAtOnce = 32;
 struct Halves
 {
@@ -445,23 +446,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                     tc::fence_async_shared();
                     __syncwarp();
                     if (lane == 0) tc::barrier_arrive(&sh.read[x]);
+                    unsigned v[2][8]; // (in front of the wait, which votes)
+#pragma unroll
+                    for (unsigned n = 0; n < 2; n++) Unfold::words(q[n], scale[n], v[n]);
                     if (!tc::warp_wait(&sh.used[h], h_phase ^ 1, &sh.gave_up)) goto end;
-                    if (scale[0] == Unfold::largest || scale[1] == Unfold::largest) // (here, in front of all stores: inside words it takes 4 % of the time)
-                    {
-                        scale[0] -= scale[0] == Unfold::largest, scale[1] -= scale[1] == Unfold::largest;
-                        sh.halved = 1;
-                    }
                     unsigned char *to = halves + h * kUnfoldedBytes + lane8 / 4 * kTile;
 #pragma unroll
                     for (unsigned n = 0; n < 2; n++)
                     {
                         const unsigned t = row0 + 32 * n;
-                        unsigned v[8];
-                        Unfold::words(q[n], scale[n], v);
                         // 16-byte pieces 2 l and 2 l + 1 of the row's 128 bytes, swapped in the second half so that eight lanes meet no conflict
                         unsigned char *line = to + t * 128;
                         const unsigned at = lane8 % 4 * 2, second = lane8 / 4;
-                        const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
+                        const uint4 lo = make_uint4(v[n][0], v[n][1], v[n][2], v[n][3]), hi = make_uint4(v[n][4], v[n][5], v[n][6], v[n][7]);
                         *reinterpret_cast<uint4 *>(line + (((at + second) ^ (t % 8)) * 16)) = second ? hi : lo;
                         *reinterpret_cast<uint4 *>(line + (((at + 1 - second) ^ (t % 8)) * 16)) = second ? lo : hi;
                     }
@@ -493,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block8_gradient(const __grid_co
                     tc::fence_async_shared();
                     __syncwarp();
                     if (lane == 0) tc::barrier_arrive(&sh.unfolded[h]);
+                    if (max(scale[0], scale[1]) == Unfold::largest) sh.halved = 1;
                 }
                 turn ^= 1;
                 if (++s == p.stages) s = 0, phase ^= 1;
@@ -550,7 +548,7 @@ end:
     tc::fence_after();
     // A cluster (and a block each): the sum's columns in `split` parts of 16 to 64; a CTA begins with its own. (All CTAs of the cluster go through this
     // together, whatever became of their waits.)
-    bool some = sh.halved; // in any CTA of the cluster
+    unsigned some = sh.halved;
     if (p.split > 1)
     {
         const Places at = places<Unfold>(p, first, warp % 4, lane);
@@ -565,10 +563,11 @@ end:
                 store_columns(at, v, c, p.accumulate || turn > 0);
             }
             cg::this_cluster().sync();
-            if (turn == 0) some = __any_sync(~0u, lane < p.split && *cg::this_cluster().map_shared_rank(&sh.halved, lane) != 0); // (there is another turn: its shared memory stays)
+            if (turn == 0 && lane < p.split) some |= *cg::this_cluster().map_shared_rank(&sh.halved, lane); // (there is another turn: its shared memory stays)
         }
     }
-    for (unsigned turn = 0; turn < p.split && some; turn++)
+    const bool any = __any_sync(~0u, some != 0); // (the same for all CTAs of a cluster)
+    for (unsigned turn = 0; turn < p.split && any; turn++)
     {
         if (turn == piece && !sh.gave_up)
             for (unsigned u = u0; u < p.n_groups; u += stride) add_halves<Unfold>(p, u, step0 * kRows, min(step1 * kRows, p.x.n), *reinterpret_cast<Halves *>(dys));
