@@ -166,8 +166,10 @@ __device__ __forceinline__ void store_columns(const Places &at, const float *v, 
     float *to = (c < 128 ? at.to[0] : at.to[1]) + r0 * 128;
     if (add)
     {
+        // By L2, without waiting; one thread's additions to a place stay in order. L2 takes numbers below 2^-126 for zero; read, added and written here they would
+        // stay, and a quarter of 4096 x 4096 by 4096 rows would take 51.6 us instead of 45.4, 300 rows added to 1024 blocks 43 instead of 24.
 #pragma unroll
-        for (unsigned k = 0; k < 16; k++) // (by L2, without waiting; one thread's additions to a place stay in order)
+        for (unsigned k = 0; k < 16; k++)
             if (r0 + k < rows) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to + k * 128), "f"(v[k]) : "memory");
     }
     else

@@ -81,6 +81,41 @@ def test_gradient_where_dy_is_not_finite(asp_ctx, blocks, columns, n, pad, dtype
     assert_gradient(torch.where(finite > 0, out, 0.0), clean, xq, p)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("blocks,columns,n,pad", WAYS)
+def test_gradient_added_to_what_is_there(asp_ctx, blocks, columns, n, pad, dtype):
+    x, dy = factors(blocks, columns, n, pad, dtype)
+    before = torch.randn(blocks * columns, 128, 128, generator=gen(5), device="cuda") * 100.0
+    once, p = gradient(asp_ctx, blocks, columns, x, dy, dtype)
+    out, _ = gradient(asp_ctx, blocks, columns, x, dy, dtype, before)
+    want = ref.rows_in_8_bits(x)
+    gradient_of = ref.stored(p, dy.double().T @ want)
+    size = ref.stored(p, dy.double().abs().T @ want.abs())
+    inside = ref.stored(p, torch.ones(dy.shape[1], x.shape[1], dtype=torch.float64, device="cuda")) > 0
+    # the sum's own roundings, and one for each of its parts that is added to what is there (parts of at least 768 rows, and 8 at most that share them)
+    parts = n // 768 + 9
+    room = size * ((n + 1) * 2.0**-23) + parts * (before.double().abs() + size) * 2.0**-24
+    assert ((out.double() - before.double() - gradient_of).abs() <= room)[inside].all()
+    assert torch.equal(out[~inside], before[~inside]) and (once[~inside] == 0).all()
+
+
+@pytest.mark.parametrize("blocks,columns,n,pad", WAYS)
+def test_gradient_added_to_the_smallest_numbers(asp_ctx, blocks, columns, n, pad):
+    """Numbers below 2^-126 may count as zero where something is added to them or they are added (each time by less than 2^-126), and nothing more is lost."""
+    x, dy = factors(blocks, columns, n, pad, "bf16")
+    n_rows = dy.shape[1]
+    before = torch.randint(-40, 41, (blocks * columns, 128, 128), generator=gen(5), device="cuda").float() * 2.0**-130
+    dy *= 0.0
+    dy[0, : n_rows // 2] = 2.0**-40  # (the other rows of the blocks: nothing is added)
+    x[0] = 2.0**-80
+    out, p = gradient(asp_ctx, blocks, columns, x, dy, "bf16", before)
+    added = ref.stored(p, dy.double().T @ ref.rows_in_8_bits(x))
+    want = before.double() + added
+    assert ((out.double() - want).abs() < 2.0**-126).all()
+    kept = (before.abs() >= 2.0**-126) | (before == 0)
+    assert torch.equal(out[kept].double(), want[kept].float().double()) and kept.any() and not kept.all()
+
+
 @pytest.mark.parametrize("rows_of_blocks,columns", [(3, 5), (40, 50)])
 def test_transposed_blocks_are_zero_until_they_have_values(asp_ctx, rows_of_blocks, columns):
     """Whatever the context has copied to the device before: here a matrix without a zero among its values."""
