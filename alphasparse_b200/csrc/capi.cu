@@ -515,7 +515,17 @@ asp_status asp_ctx_create(int device, asp_ctx **out)
         e = cudaStreamCreateWithFlags(&c->aux[i], cudaStreamNonBlocking);
         if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->ev_join[i], cudaEventDisableTiming);
     }
-    if (e == cudaSuccess) e = cudaHostAlloc((void **)&c->fault, sizeof(*c->fault), cudaHostAllocPortable | cudaHostAllocMapped);
+    if (e == cudaSuccess)
+    {
+        // (an allocation would end a capture that some stream is in, and fail; it has nothing to do with it)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        e = cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e == cudaSuccess)
+        {
+            e = cudaHostAlloc((void **)&c->fault, sizeof(*c->fault), cudaHostAllocPortable | cudaHostAllocMapped);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+        }
+    }
     if (e == cudaSuccess) *c->fault = 0;
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&c->max_smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);

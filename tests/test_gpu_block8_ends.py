@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import block8_ref as ref
+from alphasparse_b200 import capi
 from alphasparse_b200.block8 import Block8, Rows8
 from test_gpu_block8 import TYPES, assert_gradient, gen, pattern, rows
 
@@ -139,3 +140,24 @@ def test_transposed_blocks_are_zero_until_they_have_values(asp_ctx, rows_of_bloc
             assert (y == 0).all() and (y1 == 0).all(), (transposed, n)
             held.close()
     m.close()
+
+
+def test_contexts_are_made_while_another_stream_is_captured():
+    x, made = torch.zeros(8, device="cuda"), []
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        x.add_(1.0)
+        made.append(capi.Context(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (x == 1.0).all()
+    ctx = made[0]
+    m, y = Block8(ctx, 128, 128, [0, 1], [0]), torch.full((1, 128), 7.0, device="cuda")
+    rows_of_ones = torch.ones(1, 128, device="cuda")
+    torch.cuda.synchronize()
+    m.apply(rows_of_ones.data_ptr(), 1, "f32", y.data_ptr(), "f32")
+    ctx.synchronize()
+    assert (y == 0.0).all()
+    m.close()
+    ctx.close()
