@@ -31,12 +31,12 @@ __device__ __forceinline__ float power(unsigned scale) { return __uint_as_float(
 __device__ __forceinline__ float inverse(unsigned scale) { return __uint_as_float((254u - scale) << 23); } // 2^-k; scale is 1 to 247
 
 // Two elements to e4m3, `a` in the low byte; NaN stays NaN. The conversion saturates: where an element may be infinite it is made NaN first
-// (v - v is NaN then, else 0).
+// (v - v is NaN then, else 0, taken with a minus so that -0 stays -0 wherever it stands).
 template <bool infinite> __device__ __forceinline__ unsigned pack2(float a, float b, float inv)
 {
     unsigned short r;
-    a = infinite ? __fmaf_rn(a, inv, a - a) : a * inv;
-    b = infinite ? __fmaf_rn(b, inv, b - b) : b * inv;
+    a = infinite ? __fmaf_rn(a, inv, -(a - a)) : a * inv;
+    b = infinite ? __fmaf_rn(b, inv, -(b - b)) : b * inv;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
     return r;
 }

@@ -117,6 +117,31 @@ def test_gradient_added_to_the_smallest_numbers(asp_ctx, blocks, columns, n, pad
     assert torch.equal(out[kept].double(), want[kept].float().double()) and kept.any() and not kept.all()
 
 
+def same_bits(a, b):
+    return torch.equal(a.contiguous().view(torch.int32), b.contiguous().view(torch.int32))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_zeros_keep_their_sign_whatever_is_beside_them(asp_ctx, dtype):
+    x = torch.zeros(20, 512, dtype=TYPES[dtype], device="cuda")
+    x[:, ::3] = -0.0
+    x[5:, 7], x[10:, 200] = float("inf"), 3.0
+    held, out = Rows8(asp_ctx, 20, 512), torch.empty(20, 512, device="cuda")
+    m, blocks = Block8(asp_ctx, 128, 640, [0, 5], range(5)), torch.empty(5, 128, 128, device="cuda")
+    values = x.flatten().repeat(8)[: 5 * 128 * 128].contiguous()
+    torch.cuda.synchronize()
+    held.quantize(x.data_ptr(), 20, dtype)
+    held.restore(out.data_ptr(), "f32")
+    m.set_values(values.data_ptr(), dtype)
+    m.get_values(blocks.data_ptr())
+    asp_ctx.synchronize()
+    zero = x == 0
+    assert same_bits(out[zero], x.float()[zero])
+    assert same_bits(blocks.flatten()[values == 0], values.float()[values == 0])
+    held.close()
+    m.close()
+
+
 @pytest.mark.parametrize("rows_of_blocks,columns", [(3, 5), (40, 50)])
 def test_transposed_blocks_are_zero_until_they_have_values(asp_ctx, rows_of_blocks, columns):
     """Whatever the context has copied to the device before: here a matrix without a zero among its values."""
