@@ -115,8 +115,11 @@ class Block8:
     the blocks by block row, as in CSR. transposed: products with the transposed matrix are wanted, too."""
 
     def __init__(self, ctx: capi.Context, n_rows: int, n_cols: int, block_ptr, block_col, transposed: bool = False):
-        ptr = np.ascontiguousarray(block_ptr, dtype=np.int64)
-        col = np.asarray(block_col)
+        ptr, col = np.asarray(block_ptr), np.asarray(block_col)
+        for a in (ptr, col):
+            if a.dtype.kind not in "iu" and a.size and not (a.dtype.kind in "bf" and np.isfinite(a).all() and (a == np.trunc(a)).all()):
+                raise ValueError("block_ptr, block_col: whole numbers")
+        ptr = np.ascontiguousarray(ptr, dtype=np.int64)
         if col.size and (col.min() < 0 or col.max() >= 2**32):
             raise ValueError("block_col: block columns")
         col = np.ascontiguousarray(col, dtype=np.uint32)
