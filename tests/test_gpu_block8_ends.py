@@ -84,6 +84,30 @@ def test_gradient_where_dy_is_not_finite(asp_ctx, blocks, columns, n, pad, dtype
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("blocks,columns,n,pad", WAYS)
+def test_gradient_of_scales_of_all_sizes(asp_ctx, blocks, columns, n, pad, dtype):
+    """Blocks of subnormal numbers, and of numbers far above what 8 bits hold without a scale.
+
+    What is cut off goes by the exponents of the factors as they are stored, and a subnormal number has that of the smallest normal one, N: where x is j 2^-24 in fp16,
+    dy x counts as one of size 2^-14 |dy|. (-16.1875 * 2^-24 in fp16, 2^-20 in size, has the exponent 4 - 14 = -10 and made a sum be 2^-34.8 off, a step of 2^-24 below
+    that exponent; 71 rows of 2^-23 of its own size were 2^-36.) So a sum is within (n + 1) * 2^-23 * sum max(|dy|, N) max(|x|, N), factors of zero left out."""
+    x, dy = factors(blocks, columns, n, pad, dtype)
+    low, high = (-24, 15) if dtype == "f16" else (-133, 100)
+    size = torch.exp2(torch.randint(low, high + 1, (n, columns), generator=gen(8), device="cuda").double()).repeat_interleave(128, 1)[:, : x.shape[1]]
+    x = (torch.randint(-15, 16, x.shape, generator=gen(9), device="cuda").double() / 8 * size).to(TYPES[dtype])
+    least = torch.finfo(TYPES[dtype]).tiny
+    for part, factor in ((x, 2.0**-20), (torch.where(size <= 2.0 ** (low + 12), x, torch.zeros_like(x)), 2.0**80)):
+        dy *= factor if dtype == "bf16" else 1.0
+        out, p = gradient(asp_ctx, blocks, columns, part, dy, dtype)
+        xq, dyd = ref.rows_in_8_bits(part), dy.double()
+        assert torch.equal(xq.to(TYPES[dtype]).double(), xq) and (xq != 0).any()
+        want = ref.stored(p, dyd.T @ xq)
+        sizes = ref.stored(p, torch.where(dyd != 0, dyd.abs().clamp(min=least), 0.0).T @ torch.where(xq != 0, xq.abs().clamp(min=least), 0.0))
+        room = sizes * ((n + 1) * 2.0**-23) + want.abs() * 2.0**-24 + 2.0**-126
+        assert ((out.double() - want).abs() <= room).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("blocks,columns,n,pad", WAYS)
 def test_gradient_added_to_what_is_there(asp_ctx, blocks, columns, n, pad, dtype):
     x, dy = factors(blocks, columns, n, pad, dtype)
     before = torch.randn(blocks * columns, 128, 128, generator=gen(5), device="cuda") * 100.0
@@ -165,6 +189,24 @@ def test_transposed_blocks_are_zero_until_they_have_values(asp_ctx, rows_of_bloc
             assert (y == 0).all() and (y1 == 0).all(), (transposed, n)
             held.close()
     m.close()
+
+
+@pytest.mark.parametrize("dtype,rows_a_sum", [("bf16", 1280), ("f16", 768)])
+@pytest.mark.parametrize("blocks,columns,n,pad", [(1, 150, 9000, 0), (2, 100, 9000, 0), (1, 2, 9000, 0), (2, 3, 9000, 1), (3, 70, 9000, 1)])
+def test_long_sums_of_gradients_are_rounded(asp_ctx, blocks, columns, n, pad, dtype, rows_a_sum):
+    """Products of one sign. A tensor core cuts off less than 2^-23 of the sum each time it adds (16 rows): to a sum that grows evenly, over 1280 (768) rows, less than
+    (80 + 1) / 2 (24.5) times 2^-23; the sums are added up with half a step each. Sums that are shared by up to 8 CTAs are shorter, and as many more are added.
+    (All 9000 rows in one sum came to 55 and 201 times 2^-23.)"""
+    g = gen(n)
+    n_rows, n_cols = 128 * blocks - 8, 128 * columns - 5
+    x = (torch.rand(n, n_cols, generator=g, device="cuda") + 0.5).to(TYPES[dtype])
+    dy = (torch.rand(n, n_rows + (8 if pad == 0 else pad), generator=g, device="cuda") + 0.5).to(TYPES[dtype])[:, :n_rows]
+    out, p = gradient(asp_ctx, blocks, columns, x, dy, dtype)
+    want = ref.stored(p, dy.double().T @ ref.rows_in_8_bits(x))
+    inside = want > 0
+    sums = -(-n // rows_a_sum) + 8
+    off = ((out.double() - want).abs() / want)[inside].max().item()
+    assert off < ((rows_a_sum / 16 + 1) / 2 + sums / 2) * 2.0**-23, off * 2.0**23
 
 
 def test_contexts_are_made_while_another_stream_is_captured():
