@@ -29,7 +29,7 @@ typedef enum asp_status
     ASP_ERR_ALLOC = 4,       /* host or device allocation failed                            */
     ASP_ERR_BOUNDS = 5,      /* a format array refers outside val/col/x/y                   */
     ASP_ERR_IMPLAUSIBLE = 6, /* measured throughput above the configured sanity bound       */
-    ASP_ERR_TIMEOUT = 7      /* a bounded wait on the device expired (asp_dist_status)      */
+    ASP_ERR_TIMEOUT = 7      /* a bounded wait on the device expired (asp_dist_status, asp_synchronize) */
 } asp_status;
 
 /* element types of format arrays; the reference narrows every index array to the smallest

@@ -228,3 +228,47 @@ def test_contexts_are_made_while_another_stream_is_captured():
     assert (y == 0.0).all()
     m.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("blocks,columns,n,pad", WAYS)
+def test_gradient_of_the_largest_numbers_added_replayed_and_beside_another(asp_ctx, blocks, columns, n, pad, dtype):
+    x, dy = factors(blocks, columns, n, pad, dtype)
+    x = with_largest(x, dtype, 0.1)
+    if dtype == "bf16":
+        dy *= 2.0**-30
+    want = ref.rows_in_8_bits(x)
+    once, p = gradient(asp_ctx, blocks, columns, x, dy, dtype)
+    other = capi.Context(0)
+    sets = []
+    for ctx in (asp_ctx, other):
+        m, held = Block8(ctx, dy.shape[1], x.shape[1], *p), Rows8(ctx, n, x.shape[1])
+        sets.append((ctx, m, held, torch.full_like(once, 7.0)))
+    torch.cuda.synchronize()
+    for k in range(3):  # both at once
+        for ctx, m, held, out in sets:
+            held.quantize(x.data_ptr(), n, dtype)
+            m.gradient(held, dy.data_ptr(), dtype, out.data_ptr(), dy.stride(0))
+    for ctx, m, held, out in sets:
+        ctx.synchronize()
+        assert torch.equal(out, once)
+    # captured: set, then added to twice
+    ctx, m, held, out = sets[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(ctx.stream)):
+        held.quantize(x.data_ptr(), n, dtype)
+        m.gradient(held, dy.data_ptr(), dtype, out.data_ptr(), dy.stride(0))
+        m.gradient(held, dy.data_ptr(), dtype, out.data_ptr(), dy.stride(0), accumulate=True)
+    for _ in range(2):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        sizes = ref.stored(p, dy.double().abs().T @ want.abs())
+        parts = n // 768 + 10  # that are added to what is there, half a step each
+        assert ((out.double() - 2 * once.double()).abs() <= sizes * (2 * (n + 1) + parts) * 2.0**-23 + 2.0**-126).all()
+    del graph
+    for ctx, m, held, out in sets:
+        m.close()
+        held.close()
+    other.close()
