@@ -26,7 +26,7 @@ using namespace block8;
 // What bounds it is shared memory, 128 bytes a clock and SM: for 64 rows t, x of a block column passes it four times (8 KB in, 8 out, unfolded 16 in and
 // with each product 16 out), dy of a block row twice and more. Two blocks of a column share x: 56 KB a block instead of 80 for one alone, 448 clocks
 // where the products take 256. (Four would be 384, but leave no room for a second D: measured the same, with the rows below in one sum.) A quarter of
-// 4096 x 4096 by 4096 rows in bf16: 42.3 us, 815 TFLOP/s; of 8192 x 4096 by 8192: 161 us, 855 TFLOP/s, and 184 over and over, at the power limit.
+// 4096 x 4096 by 4096 rows in bf16: 42.6 us, 806 TFLOP/s; of 8192 x 4096 by 8192: 164 us, 838 TFLOP/s, and 187 in a training step, at the power limit.
 //
 // Tensor cores cut off what they add up to, which over 8192 rows in one sum showed as 6.5e-6 of the result, where sums that are rounded have 6e-7. So D takes
 // 1280 rows in bf16 (8e-7), 768 in fp16, whose products have more bits (8e-7; 1.4e-6 with 1280), then another one the next, while the first is added,
@@ -36,7 +36,7 @@ using namespace block8;
 //
 // 8 bits round up: the largest numbers of either 16-bit type become 256 times the largest scale, 2^16 or 2^128, which the type does not have. Rows with that scale
 // are unfolded to half of what they are, and a CTA that has met some adds the other half when it is done with its groups (add_halves). (A second pass of such steps through
-// the tensor cores has the issuing warp look at each step whether there are any, between two waits: 48.1 us instead of 45.4 for the quarter of 4096 x 4096, without any.)
+// the tensor cores has the issuing warp look at each step whether there are any, between two waits: 48.1 us instead of 45.4 for 243 blocks of 4096 x 4096 and 4096 rows, without any.)
 //
 // Warp 0 copies, warp 1 issues products, warps 4 to 11 add up and store, warps 12 to 19 and 20 to 27 unfold x, every second step each.
 constexpr unsigned kRows = host::kBlock8GradientRows; // t a step
@@ -50,8 +50,8 @@ constexpr unsigned kUnfolded = 3, kUnfoldedBytes = 2 * kTile; // x in 16 bits: 6
 constexpr unsigned kThreads = 896;
 constexpr size_t kSharedBytes = kRoom * kBlockBytes + kUnfolded * kUnfoldedBytes + kHeld * kHeldBytes + 1024;
 // Rows of dy that are not all on 16-byte boundaries cannot be copied by tiles. The warps that unfold x bring them, one of their steps ahead, in the aligned
-// pieces of 16 bytes that they lie in, and shift them to where they belong: 4001 rows, a quarter of 4001 x 4003, take 122 us (450 element by
-// element) where 4096 rows of 4096 x 4096 take 42 by tiles. They then take a part of dy's room, and groups are single blocks.
+// pieces of 16 bytes that they lie in, and shift them to where they belong: 4001 rows, a quarter of 4001 x 4003, take 125 us (450 element by
+// element) where 4096 rows of 4096 x 4096 take 43 by tiles. They then take a part of dy's room, and groups are single blocks.
 constexpr unsigned kPitch = 272, kRawBytes = kRows * kPitch, kShiftedStages = 3; // 17 pieces a row
 static_assert(kShiftedStages * kBlockBytes + 4 * kRawBytes <= kRoom * kBlockBytes, "two steps of each group of warps beside the stages");
 
@@ -167,7 +167,7 @@ __device__ __forceinline__ void store_columns(const Places &at, const float *v, 
     if (add)
     {
         // By L2, without waiting; one thread's additions to a place stay in order. L2 takes numbers below 2^-126 for zero; read, added and written here they would
-        // stay, and a quarter of 4096 x 4096 by 4096 rows would take 51.6 us instead of 45.4, 300 rows added to 1024 blocks 43 instead of 24.
+        // stay, and 243 blocks of 4096 x 4096 and 4096 rows would take 51.6 us instead of 45.4, 300 rows added to 1024 blocks 43 instead of 24.
 #pragma unroll
         for (unsigned k = 0; k < 16; k++)
             if (r0 + k < rows) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to + k * 128), "f"(v[k]) : "memory");
@@ -181,7 +181,7 @@ __device__ __forceinline__ void store_columns(const Places &at, const float *v, 
 
 // The other half of the rows with the largest scale, to the result of a group, by the whole CTA: 32 such rows at a time come to shared memory as 32-bit numbers, and a
 // thread multiplies and adds for 4 columns of every 28th row of a block, in the order of the rows: the same bits every time.
-// A quarter of 4096 x 4096 by 4096 rows: 45.4 us without such rows (44.2 without the test for them and the votes of waits), 65 with one, 89 with 64 in one block column, 1640 where all are in one.
+// 243 blocks of 4096 x 4096 and 4096 rows: 45.4 us without such rows (44.2 without the test for them and the votes of waits), 65 with one, 89 with 64 in one block column, 1640 where all are in one.
 constexpr unsigned kWarps = kThreads / 32, kHalvesAtOnce = 32;
 struct Halves
 {

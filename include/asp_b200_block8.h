@@ -88,7 +88,7 @@ asp_status asp_block8_product(asp_ctx *ctx, const asp_block8 *m, int transposed,
  * dA[block (i, j)] = sum over the rows of dy[128 i + .] x[128 j + .]^T, 32 bits, in the order of asp_block8_set_values; zero outside the
  * matrix. dY: ASP_F16 | ASP_BF16, the type that x was converted from (ASP_ERR_UNSUPPORTED otherwise), so that the products' factors
  * are exact; as many rows as x holds. What 8 bits have made of the type's largest numbers, 2^16 or 2^128, counts as that, although the type does not have it: rows
- * with numbers above 57344 (fp16) or 1.75 * 2^127 (bf16) take some ten times as long as others. Rows of dY on 16-byte boundaries (d_dy, and ld a multiple of 8) are copied by tiles, others take up to three times as
+ * with numbers above 57344 (fp16) or 1.75 * 2^127 (bf16) take some forty times as long as others. Rows of dY on 16-byte boundaries (d_dy, and ld a multiple of 8) are copied by tiles, others take up to three times as
  * long. accumulate != 0: added to d_out. d_out 16-byte aligned. Sums of at most 1280 rows are added up, rounded, in one order; numbers below
  * 2^-126, in d_out or among these sums, may count as zero where something is added (L2 adds them up). */
 asp_status asp_block8_gradient(asp_ctx *ctx, const asp_block8 *m, const asp_rows8 *x, const void *d_dy, int dtype, uint64_t ld, float *d_out, int accumulate);
